@@ -50,7 +50,8 @@ def lib():
     for name in ("bpl_build_twouint_onebool_descriptor", "bpl_build_double_size_descriptor",
                  "bpl_build_nonzero_descriptor", "bpl_build_jitconn_prob_homo_descriptor",
                  "bpl_build_jitconn_prob_uniform_descriptor", "bpl_build_jitconn_prob_normal_descriptor",
-                 "bpl_build_matmat_jit_prob_descriptor1"):
+                 "bpl_build_matmat_jit_prob_descriptor1", "bpl_build_expert_descriptor",
+                 "bpl_expert_sort_scratch_bytes"):
       getattr(l, name).restype = ctypes.c_size_t
     _lib = l
   return _lib
@@ -224,3 +225,15 @@ def build_matmat_jit_prob_descriptor1(m, k, n, seed, log_p, w1, w2):
   return _build("bpl_build_matmat_jit_prob_descriptor1", ctypes.c_uint32(m), ctypes.c_uint32(k),
                 ctypes.c_uint32(n), ctypes.c_uint32(seed & 0xFFFFFFFF), ctypes.c_double(log_p),
                 ctypes.c_double(w1), ctypes.c_double(w2))
+
+
+@functools.lru_cache(maxsize=256)
+def build_expert_descriptor(tokens, per_token, experts, rows, width, out_width, flags):
+  u = ctypes.c_uint32
+  return _build("bpl_build_expert_descriptor", u(tokens), u(per_token), u(experts), u(rows), u(width), u(out_width),
+                u(flags))
+
+
+@functools.lru_cache(maxsize=256)
+def expert_sort_scratch_bytes(pairs, experts):
+  return lib().bpl_expert_sort_scratch_bytes(ctypes.c_uint32(pairs), ctypes.c_uint32(experts))

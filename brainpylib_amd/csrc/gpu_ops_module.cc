@@ -85,6 +85,11 @@ PYBIND11_MODULE(gpu_ops, m) {
           return BPL_PACK(bpl_build_event_csr_batching_descriptor, n_row, n_col, batch_size, values_batch,
                           indices_batch, indptr_batch, events_batch, nnz, transpose ? 1 : 0);
         });
+  m.def("build_expert_descriptor",
+        [](uint32_t tokens, uint32_t per_token, uint32_t experts, uint32_t rows, uint32_t width, uint32_t out_width,
+           uint32_t flags) {
+          return BPL_PACK(bpl_build_expert_descriptor, tokens, per_token, experts, rows, width, out_width, flags);
+        });
   m.def("build_csr_event_sum_descriptor",
         [](uint32_t pre_size, uint32_t post_size) { return BPL_PACK(bpl_build_csr_event_sum_descriptor, pre_size, post_size); });
   m.def("build_coo_event_sum_descriptor",

@@ -216,6 +216,7 @@ static_assert(sizeof(bpl_jitconn_prob_weight_descriptor) == 40, "JITConnProb{Uni
 static_assert(offsetof(bpl_jitconn_prob_weight_descriptor, w_a) == 24, "w_a at offset 24");
 static_assert(sizeof(bpl_matmat_jit_prob_descriptor) == 40, "MatMatJITProbDescriptor1 is 40 bytes");
 static_assert(offsetof(bpl_matmat_jit_prob_descriptor, log_p) == 16, "log_p at offset 16");
+static_assert(sizeof(bpl_expert_descriptor) == 28, "the expert descriptor is 28 bytes");
 
 namespace {
 template <typename T>
@@ -341,6 +342,12 @@ size_t bpl_build_matmat_jit_prob_descriptor1(uint32_t m, uint32_t k, uint32_t n,
   d.log_p = log_p;
   d.w_a = w_a;
   d.w_b = w_b;
+  return pack(d, out, cap);
+}
+
+size_t bpl_build_expert_descriptor(uint32_t tokens, uint32_t per_token, uint32_t experts, uint32_t rows, uint32_t width,
+                                   uint32_t out_width, uint32_t flags, char *out, size_t cap) {
+  bpl_expert_descriptor d{tokens, per_token, experts, rows, width, out_width, flags};
   return pack(d, out, cap);
 }
 

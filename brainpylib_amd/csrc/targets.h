@@ -150,6 +150,33 @@
   X(gpu_csr_event_prod_heter_f64_i32) \
   X(gpu_csr_event_prod_heter_f64_i64)
 
+#define BPL_EXPERT_TARGETS(X) \
+  X(expert_topk_float) \
+  X(expert_topk_half) \
+  X(expert_topk_bfloat16) \
+  X(expert_topk_gradient_float) \
+  X(expert_topk_gradient_half) \
+  X(expert_topk_gradient_bfloat16) \
+  X(expert_sort) \
+  X(expert_dispatch_float) \
+  X(expert_dispatch_half) \
+  X(expert_dispatch_bfloat16) \
+  X(expert_dispatch_gradient_float) \
+  X(expert_dispatch_gradient_half) \
+  X(expert_dispatch_gradient_bfloat16) \
+  X(expert_combine_float) \
+  X(expert_combine_half) \
+  X(expert_combine_bfloat16) \
+  X(expert_combine_gradient_float) \
+  X(expert_combine_gradient_half) \
+  X(expert_combine_gradient_bfloat16) \
+  X(expert_matmul_float) \
+  X(expert_matmul_half) \
+  X(expert_matmul_bfloat16) \
+  X(expert_matmul_gradient_float) \
+  X(expert_matmul_gradient_half) \
+  X(expert_matmul_gradient_bfloat16)
+
 #define BPL_ALL_TARGETS(X)  \
   BPL_EVENT_CSR_TARGETS(X)  \
   BPL_EVENT_CSR_BATCHING_TARGETS(X) \
@@ -158,4 +185,5 @@
   BPL_JITCONN_HASH_TARGETS(X) \
   BPL_MATMAT_TARGETS(X)     \
   BPL_NONZERO_TARGETS(X)    \
-  BPL_COMPAT_TARGETS(X)
+  BPL_COMPAT_TARGETS(X)     \
+  BPL_EXPERT_TARGETS(X)

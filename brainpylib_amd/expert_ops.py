@@ -1,0 +1,393 @@
+"""Routing of tokens to experts, and the experts' products (host side).
+
+A mixture of experts is a network of which every token meets only a few parts: the routing is a sparse tokens x experts
+matrix with ``k`` nonzeros a row, its index arrays are built on the GPU as ``coo_to_csr`` builds those of synapses, and
+only the products that it names are computed.  The reference has no such operators.
+
+    weights, experts = expert_topk(logits, k=k)                       # the nonzeros of every row
+    indptr, order, position = expert_sort(experts, num_experts=n)     # the same by expert
+    rows = expert_dispatch(tokens, order, position)                   # a row for every nonzero, sorted by expert
+    rows = expert_matmul(rows, weight, indptr)                        # every expert's rows times its matrix
+    out = expert_combine(rows, weights, order, position)              # the weighted sum of every token's rows
+
+Values are float32, float16 or bfloat16; sums, softmax and routing weights are held in 32 bits.  Gradients are of first
+order, in backward mode.  No call waits for the GPU or reads a count back, so all of them can be captured into a HIP graph;
+none uses scratch memory that outlives it, so graphs share none.  Results do not depend on the order of atomics.
+"""
+import torch
+
+from . import _lib
+from ._tensors import as_tensor, device_of, has_tangent, is_index_dtype, keep_signature, to_device
+
+__all__ = ["expert_topk", "expert_sort", "expert_dispatch", "expert_combine", "expert_matmul"]
+
+_TYPE_NAME = {torch.float32: '_float', torch.float16: '_half', torch.bfloat16: '_bfloat16'}
+_NORMALIZE, _MASKED, _OUT_MAJOR, _D_ROWS, _D_WEIGHTS = 1, 2, 4, 8, 16  # BPL_EXPERT_* of the descriptor
+_MOST_EXPERTS, _MOST_PER_TOKEN, _MOST = 1024, 64, 2 ** 31 - 1
+
+
+def _call(name, buffers, opaque):
+  device = buffers[0].device
+  if device.index == torch.cuda.current_device():
+    _lib.custom_call(name, buffers, opaque)
+  else:  # (a kernel is launched on the current device, whatever the stream's)
+    with torch.cuda.device(device):
+      _lib.custom_call(name, buffers, opaque)
+
+
+def _move(*tensors):
+  device = device_of(*tensors)
+  return [to_device(t, device) for t in tensors]
+
+
+def _check_values(name, t, ndim):
+  if t.dtype not in _TYPE_NAME:
+    raise TypeError(f'Only support float32, float16 and bfloat16. But we got {t.dtype} for {name}.')
+  if t.ndim != ndim:
+    raise ValueError(f'{name} should be a {ndim}D array. But we got {t.ndim}-D array.')
+  if max(t.shape, default=0) > _MOST:
+    raise ValueError(f'{name} should have at most 2^31 - 1 entries in each dimension, got {tuple(t.shape)}.')
+
+
+def _check_index(name, t, ndim):
+  if not is_index_dtype(t.dtype):
+    raise ValueError(f'{name} should have int32 or uint32 type, got {t.dtype}.')
+  if t.ndim != ndim:
+    raise ValueError(f'{name} should be a {ndim}D array. But we got {t.ndim}-D array.')
+
+
+def _check_pairs(order, position, tokens):
+  _check_index('order', order, 1)
+  _check_index('position', position, 2)
+  if position.shape[0] != tokens:
+    raise ValueError(f'position should have a row for each of the {tokens} tokens, got {tuple(position.shape)}.')
+  if position.shape[1] > _MOST_PER_TOKEN:
+    raise ValueError(f'Only support up to {_MOST_PER_TOKEN} experts a token, got {position.shape[1]}.')
+  if order.shape[0] != position.numel():
+    raise ValueError(f'order should have an entry for each entry of position, got {order.shape[0]} != {position.numel()}.')
+  if position.numel() > _MOST:
+    raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
+
+
+def _check_experts(n):
+  if not 1 <= n <= _MOST_EXPERTS:
+    raise ValueError(f'Only support 1 to {_MOST_EXPERTS} experts, got {n}.')
+
+
+def _differentiable(name, *tensors):
+  """Whether a gradient is asked for; tangents are refused."""
+  for t in tensors:
+    if has_tangent(t):
+      raise NotImplementedError(f'{name} has no forward-mode differentiation.')
+  return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+class _FirstOrder(torch.autograd.Function):
+  """A gradient, unchanged, of which no gradient can be had: it takes part in the graph of what it was computed from."""
+
+  @staticmethod
+  def forward(ctx, name, grad, *sources):
+    ctx.name = name
+    return grad.view_as(grad)
+
+  @staticmethod
+  def backward(ctx, ct):
+    raise NotImplementedError(f'{ctx.name} has gradients of first order only.')
+
+
+def _cotangent(name, ct):
+  if has_tangent(ct):
+    raise NotImplementedError(f'{name} has no forward-mode differentiation.')
+  return ct.detach().contiguous()
+
+
+def _first_order(name, grad, *sources):
+  if grad is not None and torch.is_grad_enabled() and any(t.requires_grad for t in sources):  # (create_graph)
+    return _FirstOrder.apply(name, grad, *sources)
+  return grad
+
+
+# ---- expert_topk ------------------------------------------------------------------------------------------------------
+def _topk(logits, mask, k, normalize):
+  n, experts = logits.shape
+  weights = torch.empty((n, k), dtype=torch.float32, device=logits.device)
+  chosen = torch.empty((n, k), dtype=torch.int32, device=logits.device)
+  flags = (_NORMALIZE if normalize else 0) | (0 if mask is None else _MASKED)
+  opaque = _lib.build_expert_descriptor(n, k, experts, 0, 0, 0, flags)
+  _call('expert_topk' + _TYPE_NAME[logits.dtype], [logits, logits if mask is None else mask, weights, chosen], opaque)
+  return weights, chosen
+
+
+@keep_signature
+class _ExpertTopk(torch.autograd.Function):
+  """With w the weights, g their cotangent: normalized, the chosen logits' cotangents are w (g - sum w g) and the others'
+  0; else, with p the softmax over all experts, p ([chosen] g - sum w g)."""
+
+  @staticmethod
+  def forward(logits, mask, k, normalize):
+    return _topk(logits, mask, k, normalize)
+
+  @staticmethod
+  def setup_context(ctx, inputs, output):
+    logits, _, ctx.k, ctx.normalize = inputs
+    weights, chosen = output
+    ctx.mark_non_differentiable(chosen)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, weights, chosen)
+
+  @staticmethod
+  def backward(ctx, ct, _):
+    if ct is None:
+      return None, None, None, None
+    logits, weights, chosen = ctx.saved_tensors
+    given, ct = ct, _cotangent('expert_topk', ct)
+    grad = torch.empty_like(logits)
+    opaque = _lib.build_expert_descriptor(logits.shape[0], ctx.k, logits.shape[1], 0, 0, 0, _NORMALIZE if ctx.normalize else 0)
+    _call('expert_topk_gradient' + _TYPE_NAME[logits.dtype], [logits, chosen, weights, ct, grad], opaque)
+    return _first_order('expert_topk', grad, given, logits), None, None, None
+
+
+def expert_topk(logits, *, k: int, normalize: bool = True, mask=None):
+  """Chooses ``k`` experts for every token.
+
+  logits  (tokens, experts) float32 | float16 | bfloat16, up to 1,024 experts
+  k       experts a token, 1 to min(experts, 64)
+  mask    (tokens,) bool, False for rows of padding; None: there are none
+  returns ``(weights, experts)``: float32 and int32 of shape (tokens, k), the largest logit first and the lowest index
+          first among equal ones.  The weights are the softmax over the chosen experts (``normalize``), or theirs of the
+          softmax over all.
+
+  A logit of -inf is never chosen; places that are left over, and all those of a row of padding, hold expert -1 and weight 0,
+  and have no gradient.  The lowest finite value is a logit like any other.  NaN counts as larger than every number and
+  makes its row's weights NaN."""
+  logits = as_tensor(logits)
+  _check_values('logits', logits, 2)
+  _check_experts(logits.shape[1])
+  if not 1 <= k <= min(logits.shape[1], _MOST_PER_TOKEN):
+    raise ValueError(f'k should be 1 to {min(logits.shape[1], _MOST_PER_TOKEN)}, got {k}.')
+  if logits.shape[0] * k > _MOST:
+    raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
+  if mask is None:
+    logits, = _move(logits)
+  else:
+    mask = as_tensor(mask)
+    if mask.dtype != torch.bool or tuple(mask.shape) != (logits.shape[0],):
+      raise ValueError(f'mask should be a bool for each of the {logits.shape[0]} tokens, got {mask.dtype} {tuple(mask.shape)}.')
+    logits, mask = _move(logits, mask)
+  if _differentiable('expert_topk', logits):
+    return _ExpertTopk.apply(logits, mask, int(k), bool(normalize))
+  return _topk(logits, mask, int(k), bool(normalize))
+
+
+# ---- expert_sort ------------------------------------------------------------------------------------------------------
+def expert_sort(experts, *, num_experts: int):
+  """Sorts pairs of a token and an expert by expert, in the pairs' order within one.
+
+  experts  (tokens, k) or (pairs,) int32 | uint32; what is outside [0, num_experts) is dropped
+  returns  ``(indptr, order, position)``, int32: expert ``e`` has the rows ``indptr[e]`` to ``indptr[e + 1] - 1``; row ``r``
+           holds pair ``order[r]`` (pairs are numbered row by row), -1 from row ``indptr[num_experts]`` on; pair ``p`` has row
+           ``position.reshape(-1)[p]``, -1 where it was dropped.  ``position`` has the shape of ``experts``."""
+  experts = as_tensor(experts)
+  _check_index('experts', experts, 1 if experts.ndim == 1 else 2)
+  _check_experts(num_experts)
+  pairs = experts.numel()
+  if pairs > _MOST:
+    raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
+  experts, = _move(experts)
+
+  def ints(*shape):
+    return torch.empty(shape, dtype=torch.int32, device=experts.device)
+
+  indptr, order, position = ints(num_experts + 1), ints(pairs), ints(*experts.shape)
+  scratch = ints(_lib.expert_sort_scratch_bytes(pairs, num_experts) // 4)
+  opaque = _lib.build_expert_descriptor(pairs, 1, num_experts, 0, 0, 0, 0)
+  _call('expert_sort', [experts, indptr, order, position, scratch], opaque)
+  return indptr, order, position
+
+
+# ---- expert_dispatch, expert_combine ----------------------------------------------------------------------------------
+def _pairs_opaque(position, width, flags=0):
+  return _lib.build_expert_descriptor(position.shape[0], position.shape[1], 1, 0, width, 0, flags)
+
+
+def _dispatch(tokens, order, position):
+  rows = torch.empty((order.shape[0], tokens.shape[1]), dtype=tokens.dtype, device=tokens.device)
+  _call('expert_dispatch' + _TYPE_NAME[tokens.dtype], [tokens, order, position, rows],
+        _pairs_opaque(position, tokens.shape[1]))
+  return rows
+
+
+@keep_signature
+class _ExpertDispatch(torch.autograd.Function):
+  """The cotangent of a token is the sum of its rows' cotangents."""
+
+  @staticmethod
+  def forward(tokens, order, position):
+    return _dispatch(tokens, order, position)
+
+  @staticmethod
+  def setup_context(ctx, inputs, output):
+    _, order, position = inputs
+    ctx.save_for_backward(order, position)
+    ctx.set_materialize_grads(False)
+
+  @staticmethod
+  def backward(ctx, ct):
+    if ct is None:
+      return None, None, None
+    order, position = ctx.saved_tensors
+    given, ct = ct, _cotangent('expert_dispatch', ct)
+    grad = torch.empty((position.shape[0], ct.shape[1]), dtype=ct.dtype, device=ct.device)
+    _call('expert_dispatch_gradient' + _TYPE_NAME[ct.dtype], [ct, order, position, grad],
+          _pairs_opaque(position, ct.shape[1]))
+    return _first_order('expert_dispatch', grad, given), None, None
+
+
+def expert_dispatch(tokens, order, position):
+  """The tokens' rows in the order of the experts: ``rows[position[t, i]] = tokens[t]``.
+
+  tokens    (tokens, width) float32 | float16 | bfloat16
+  order     (tokens * k,) and  position (tokens, k), as ``expert_sort`` gives them (k up to 64)
+  returns   (tokens * k, width): rows that no pair leads to (those behind the last expert's) are zero.
+
+  A pair counts only where the two arrays answer each other, ``order[position[t, i]] == t * k + i``."""
+  tokens, order, position = as_tensor(tokens), as_tensor(order), as_tensor(position)
+  _check_values('tokens', tokens, 2)
+  _check_pairs(order, position, tokens.shape[0])
+  tokens, order, position = _move(tokens, order, position)
+  if _differentiable('expert_dispatch', tokens):
+    return _ExpertDispatch.apply(tokens, order, position)
+  return _dispatch(tokens, order, position)
+
+
+def _combine(rows, weights, order, position):
+  out = torch.empty((position.shape[0], rows.shape[1]), dtype=rows.dtype, device=rows.device)
+  _call('expert_combine' + _TYPE_NAME[rows.dtype], [rows, weights, order, position, out],
+        _pairs_opaque(position, rows.shape[1]))
+  return out
+
+
+@keep_signature
+class _ExpertCombine(torch.autograd.Function):
+  """The cotangent of a row is its token's times the pair's weight, that of the weight their inner product with the row."""
+
+  @staticmethod
+  def forward(rows, weights, order, position):
+    return _combine(rows, weights, order, position)
+
+  @staticmethod
+  def setup_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+    ctx.set_materialize_grads(False)
+
+  @staticmethod
+  def backward(ctx, ct):
+    want_rows, want_weights = ctx.needs_input_grad[:2]
+    if ct is None or not (want_rows or want_weights):
+      return None, None, None, None
+    rows, weights, order, position = ctx.saved_tensors
+    given, ct = ct, _cotangent('expert_combine', ct)
+    d_rows = torch.empty_like(rows) if want_rows else None
+    d_weights = torch.empty_like(weights) if want_weights else None
+    opaque = _pairs_opaque(position, rows.shape[1], (_D_ROWS if want_rows else 0) | (_D_WEIGHTS if want_weights else 0))
+    _call('expert_combine_gradient' + _TYPE_NAME[rows.dtype],
+          [rows, weights, order, position, ct, d_rows if want_rows else rows, d_weights if want_weights else weights], opaque)
+    sources = (given, rows, weights)
+    return _first_order('expert_combine', d_rows, *sources), _first_order('expert_combine', d_weights, *sources), None, None
+
+
+def expert_combine(rows, weights, order, position):
+  """The experts' rows put together for every token: ``out[t] = sum over i of weights[t, i] * rows[position[t, i]]``.
+
+  rows      (tokens * k, width) float32 | float16 | bfloat16, sorted by expert
+  weights   (tokens, k) float32, as ``expert_topk`` gives them
+  order, position   as ``expert_sort`` gives them
+  returns   (tokens, width) of the rows' type; the sum is held in 32 bits.
+
+  Pairs that were dropped contribute nothing, whatever stands in their weight, and have gradient 0; a token without any is
+  zero."""
+  rows, weights, order, position = as_tensor(rows), as_tensor(weights), as_tensor(order), as_tensor(position)
+  _check_values('rows', rows, 2)
+  _check_pairs(order, position, position.shape[0] if position.ndim == 2 else 0)
+  if weights.dtype != torch.float32:
+    raise TypeError(f'weights should be float32, got {weights.dtype}.')
+  if weights.shape != position.shape:
+    raise ValueError(f'weights should have the shape of position, got {tuple(weights.shape)} != {tuple(position.shape)}.')
+  if rows.shape[0] != order.shape[0]:
+    raise ValueError(f'rows should have a row for each entry of order, got {rows.shape[0]} != {order.shape[0]}.')
+  rows, weights, order, position = _move(rows, weights, order, position)
+  if _differentiable('expert_combine', rows, weights):
+    return _ExpertCombine.apply(rows, weights, order, position)
+  return _combine(rows, weights, order, position)
+
+
+# ---- expert_matmul ----------------------------------------------------------------------------------------------------
+def _matmul(rows, stored, indptr, out_major):
+  """rows @ weight by expert; ``stored`` is the weight as it lies in memory, (experts, out, inner) where ``out_major``."""
+  out_width = stored.shape[1] if out_major else stored.shape[2]
+  out = torch.empty((rows.shape[0], out_width), dtype=rows.dtype, device=rows.device)
+  opaque = _lib.build_expert_descriptor(0, 0, stored.shape[0], rows.shape[0], rows.shape[1], out_width,
+                                        _OUT_MAJOR if out_major else 0)
+  _call('expert_matmul' + _TYPE_NAME[rows.dtype], [rows, stored, indptr, out], opaque)
+  return out
+
+
+@keep_signature
+class _ExpertMatmul(torch.autograd.Function):
+  """The rows' cotangent is the product with the transposed weights, the weights' is rows_e^T @ ct_e for every expert."""
+
+  @staticmethod
+  def forward(rows, stored, indptr, out_major):
+    return _matmul(rows, stored, indptr, out_major)
+
+  @staticmethod
+  def setup_context(ctx, inputs, output):
+    rows, stored, indptr, ctx.out_major = inputs
+    ctx.save_for_backward(rows, stored, indptr)
+    ctx.set_materialize_grads(False)
+
+  @staticmethod
+  def backward(ctx, ct):
+    if ct is None:
+      return None, None, None, None
+    rows, stored, indptr = ctx.saved_tensors
+    given, ct = ct, _cotangent('expert_matmul', ct)
+    d_rows = d_stored = None
+    if ctx.needs_input_grad[0]:
+      d_rows = _matmul(ct, stored, indptr, not ctx.out_major)
+    if ctx.needs_input_grad[1]:
+      d_stored = torch.empty_like(stored)
+      opaque = _lib.build_expert_descriptor(0, 0, stored.shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
+                                            _OUT_MAJOR if ctx.out_major else 0)
+      _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct, indptr, d_stored], opaque)
+    sources = (given, rows, stored)
+    return _first_order('expert_matmul', d_rows, *sources), _first_order('expert_matmul', d_stored, *sources), None, None
+
+
+def expert_matmul(rows, weight, indptr):
+  """Every expert's rows times its matrix: ``out[r] = rows[r] @ weight[e]`` for ``indptr[e] <= r < indptr[e + 1]``.
+
+  rows      (rows, inner) float32 | float16 | bfloat16, sorted by expert
+  weight    (experts, inner, out) of the rows' type, up to 1,024 experts.  Both storages are taken as they are: contiguous,
+            or the transposed view of a contiguous (experts, out, inner); its gradient is stored the same way.
+  indptr    (experts + 1,) int32 | uint32, not decreasing from 0, as ``expert_sort`` gives it
+  returns   (rows, out); rows from ``indptr[experts]`` on are zero.  Sums are held in 32 bits.
+
+  indptr is trusted to split the rows as said, as index arrays are elsewhere in the package; whatever it holds, nothing
+  outside the arrays is touched."""
+  rows, weight, indptr = as_tensor(rows), as_tensor(weight), as_tensor(indptr)
+  _check_values('rows', rows, 2)
+  _check_values('weight', weight, 3)
+  _check_index('indptr', indptr, 1)
+  if weight.dtype != rows.dtype:
+    raise TypeError(f'The types of rows and weight should be the same. But we got {rows.dtype} != {weight.dtype}.')
+  _check_experts(weight.shape[0])
+  if weight.shape[1] != rows.shape[1]:
+    raise ValueError(f'Shape mismatch, rows {tuple(rows.shape)} @ weight {tuple(weight.shape)}.')
+  if indptr.shape[0] != weight.shape[0] + 1:
+    raise ValueError(f'indptr should have experts + 1 = {weight.shape[0] + 1} entries, got {indptr.shape[0]}.')
+  out_major = not weight.is_contiguous() and weight.transpose(1, 2).is_contiguous()
+  rows, stored, indptr = _move(rows, weight.transpose(1, 2) if out_major else weight, indptr)
+  if _differentiable('expert_matmul', rows, stored):
+    return _ExpertMatmul.apply(rows, stored, indptr, out_major)
+  return _matmul(rows, stored, indptr, out_major)

@@ -138,11 +138,32 @@ typedef struct {
   double w_b;
 } bpl_matmat_jit_prob_descriptor;
 
+/* Descriptor of the expert_* targets (own targets: the reference has none of these operators).  One layout for the
+ * family; a target reads the fields that its comment names, the others are 0. */
+typedef struct {
+  uint32_t tokens;    /* T */
+  uint32_t per_token; /* k: pairs (token, expert) of one token; pair p = t * k + i */
+  uint32_t experts;   /* E, at most 1,024 */
+  uint32_t rows;      /* R: rows of the products' left operand */
+  uint32_t width;     /* elements of a token's row; the products' inner dimension K */
+  uint32_t out;       /* N: the products' columns */
+  uint32_t flags;     /* BPL_EXPERT_* */
+} bpl_expert_descriptor;
+#define BPL_EXPERT_NORMALIZE 1u /* expert_topk*: weights add up to 1 over the chosen experts */
+#define BPL_EXPERT_MASKED 2u    /* expert_topk: the mask operand is read */
+#define BPL_EXPERT_OUT_MAJOR 4u /* expert_matmul*: a weight matrix is stored [N][K] instead of [K][N] */
+#define BPL_EXPERT_D_ROWS 8u    /* expert_combine_gradient: d_rows is wanted */
+#define BPL_EXPERT_D_WEIGHTS 16u /* expert_combine_gradient: d_weights is wanted */
+
 /* Builders: write the descriptor's byte image into `out` (capacity `cap`) and return its size,
  * or 0 if `cap` is too small.  They replace build_*_descriptor of
  * lib/kernel_helper_descriptor.cu:34-104.  Unlike the reference's builders, which narrow
  * log_p and the weight parameters to float before widening them again, these keep the
  * doubles, so the kernels see the same log_p as the reference's CPU path. */
+size_t bpl_build_expert_descriptor(uint32_t tokens, uint32_t per_token, uint32_t experts, uint32_t rows, uint32_t width,
+                                   uint32_t out_width, uint32_t flags, char *out, size_t cap);
+/* Bytes of scratch memory that expert_sort of so many pairs takes as its last buffer. */
+size_t bpl_expert_sort_scratch_bytes(uint32_t pairs, uint32_t experts);
 size_t bpl_build_event_csr_batching_descriptor(uint32_t n_row, uint32_t n_col, uint32_t batch_size,
                                                uint32_t values_batch, uint32_t indices_batch,
                                                uint32_t indptr_batch, uint32_t events_batch, uint32_t nnz,
@@ -567,6 +588,61 @@ BPL_TARGET(nonzero_int);
 BPL_TARGET(nonzero_long);
 BPL_TARGET(nonzero_float);
 BPL_TARGET(nonzero_double);
+
+/* ------------------------------------------------------------------------------------------
+ * Routing of tokens to experts, and the experts' products (own targets).  T = float, half, bfloat16; weights and their
+ * gradients are float, index arrays int32; opaque = bpl_expert_descriptor.  A pair p = t * k + i has the row position[p];
+ * order[position[p]] == p.  Pairs without an expert have position -1, rows without a pair have order -1; a pair (row) whose
+ * position (order) is outside the arrays, or is not answered by the other array, counts as one without.
+ *
+ * expert_topk_T            buffers = [logits T[tokens][experts], mask uint8[tokens] (read if flagged; 0: a row of
+ *                          padding), weights float[tokens][k], chosen int32[tokens][k]]
+ *                          the k largest logits of a row, largest first, the lowest index first among equals (NaN is above
+ *                          every number); -inf is never chosen: places left over get expert -1 and weight 0, as do
+ *                          rows of padding.  weights: softmax over all experts, or, normalized, over the chosen.  k <= 64.
+ * expert_topk_gradient_T   buffers = [logits, chosen, weights, d_weights float[tokens][k], d_logits T[tokens][experts]]
+ * expert_sort              buffers = [chosen int32[tokens][k], indptr int32[experts + 1], order int32[tokens * k],
+ *                          position int32[tokens][k], scratch (bpl_expert_sort_scratch_bytes())]
+ *                          pairs sorted by expert, in the order of the pairs within one; what is outside [0, experts)
+ *                          is dropped: position -1, and order ends in -1 from indptr[experts] on.
+ * expert_dispatch_T        buffers = [tokens T[tokens][width], order, position, rows T[tokens * k][width]]
+ *                          rows[position[p]] = tokens[p / k]; rows without a pair are zero
+ * expert_dispatch_gradient_T  buffers = [d_rows, order, position, d_tokens]: the sum over a token's rows, in float
+ * expert_combine_T         buffers = [rows T[tokens * k][width], weights, order, position, out T[tokens][width]]
+ *                          out[t] = sum over i of weights[t][i] * rows[position[t][i]], in float
+ * expert_combine_gradient_T   buffers = [rows, weights, order, position, d_out, d_rows, d_weights]
+ * expert_matmul_T          buffers = [rows T[rows][width], weight T[experts][width][out] (out-major: [experts][out][width]),
+ *                          indptr int32[experts + 1], out T[rows][out]]
+ *                          out[r] = rows[r] @ weight[e] for indptr[e] <= r < indptr[e + 1] (indptr[0] is taken as 0), zero
+ *                          from indptr[experts] on; sums in float
+ * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight]: rows_e^T @ d_out_e, zero for an expert
+ *                          without rows.  (The gradient of the rows is expert_matmul with the weight's other storage.)
+ * ---------------------------------------------------------------------------------------- */
+BPL_TARGET(expert_topk_float);
+BPL_TARGET(expert_topk_half);
+BPL_TARGET(expert_topk_bfloat16);
+BPL_TARGET(expert_topk_gradient_float);
+BPL_TARGET(expert_topk_gradient_half);
+BPL_TARGET(expert_topk_gradient_bfloat16);
+BPL_TARGET(expert_sort);
+BPL_TARGET(expert_dispatch_float);
+BPL_TARGET(expert_dispatch_half);
+BPL_TARGET(expert_dispatch_bfloat16);
+BPL_TARGET(expert_dispatch_gradient_float);
+BPL_TARGET(expert_dispatch_gradient_half);
+BPL_TARGET(expert_dispatch_gradient_bfloat16);
+BPL_TARGET(expert_combine_float);
+BPL_TARGET(expert_combine_half);
+BPL_TARGET(expert_combine_bfloat16);
+BPL_TARGET(expert_combine_gradient_float);
+BPL_TARGET(expert_combine_gradient_half);
+BPL_TARGET(expert_combine_gradient_bfloat16);
+BPL_TARGET(expert_matmul_float);
+BPL_TARGET(expert_matmul_half);
+BPL_TARGET(expert_matmul_bfloat16);
+BPL_TARGET(expert_matmul_gradient_float);
+BPL_TARGET(expert_matmul_gradient_half);
+BPL_TARGET(expert_matmul_gradient_bfloat16);
 
 #ifdef __cplusplus
 } /* extern "C" */
