@@ -2,13 +2,13 @@
 // (expert_matmul_gradient).  The rows lie sorted by expert; how many an expert has is known on the device only, so the
 // grid is sized for the most tiles that any split of the rows into experts has, and a workgroup finds its tile's expert in
 // indptr.
+#include <type_traits>
+
 #include "expert.h"
 
 namespace {
 
 using namespace bpl;
-
-constexpr uint32_t kThreads = 256;
 
 // The rows of expert e, whatever indptr says within the array; e == experts: the rows behind the last.
 __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, uint32_t e, uint32_t experts, uint32_t rows) {
@@ -19,46 +19,60 @@ __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, ui
 }
 
 struct Tile {
-  uint32_t expert, first, end;  // the rows of the tile: [first, end); expert kNoTile: there is none
+  uint32_t expert, first, end;  // the rows of the tile: [first, end)
 };
-constexpr uint32_t kNoTile = 0xffffffffu;
 
-// Tile `index` of `height` rows, counted over the experts in their order and the rows behind the last: all threads of
-// the workgroup scan the experts' numbers of tiles.
-__device__ __forceinline__ Tile find_tile(const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t rows,
-                                          uint32_t height, uint32_t index) {
-  constexpr uint32_t kPer = (kMostExperts + 1 + kThreads - 1) / kThreads, kWaves = kThreads / kWave;
-  __shared__ uint32_t wave_total[kWaves];
-  __shared__ Tile found;
-  const uint32_t per = (experts + 1 + kThreads - 1) / kThreads;
-  if (threadIdx.x == 0) found.expert = kNoTile;
+// Tiles of `height` rows, counted over the experts in their order and the rows behind the last: all threads of the
+// workgroup scan the experts' numbers of tiles.
+template <uint32_t THREADS>
+struct TileFinder {
+  static constexpr uint32_t kPer = (kMostExperts + 1 + THREADS - 1) / THREADS, kWaves = THREADS / kWave;
   uint2 range[kPer];
-  uint32_t tiles = 0;
+  uint32_t before, per, height;
+
+  Tile *found;  // in LDS
+
+  __device__ __forceinline__ TileFinder(const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t rows, uint32_t height_,
+                                        uint32_t *total) : height(height_) {
+    __shared__ uint32_t wave_total[kWaves];
+    __shared__ Tile tile;
+    found = &tile;
+    if (threadIdx.x == 0) tile = Tile{experts, 0, 0};  // (nothing, should no thread find it)
+    per = (experts + 1 + THREADS - 1) / THREADS;
+    uint32_t tiles = 0;
 #pragma unroll
-  for (uint32_t j = 0; j < kPer; ++j) {
-    const uint32_t e = threadIdx.x * per + j;
-    range[j] = j < per && e <= experts ? rows_of(indptr, e, experts, rows) : make_uint2(0, 0);
-    tiles += (range[j].y - range[j].x + height - 1) / height;
-  }
-  const uint32_t upto = wave_inclusive_scan_u32(tiles);
-  if (threadIdx.x % kWave == kWave - 1) wave_total[threadIdx.x / kWave] = upto;
-  __syncthreads();
-  uint32_t before = upto - tiles;
-  for (uint32_t w = 0; w < threadIdx.x / kWave; ++w) before += wave_total[w];
-#pragma unroll
-  for (uint32_t j = 0; j < kPer; ++j) {
-    const uint32_t n = (range[j].y - range[j].x + height - 1) / height;
-    if (index >= before && index - before < n) {
-      const uint32_t first = range[j].x + (index - before) * height;
-      found.expert = threadIdx.x * per + j;
-      found.first = first;
-      found.end = range[j].y - first < height ? range[j].y : first + height;
+    for (uint32_t j = 0; j < kPer; ++j) {
+      const uint32_t e = threadIdx.x * per + j;
+      range[j] = j < per && e <= experts ? rows_of(indptr, e, experts, rows) : make_uint2(0, 0);
+      tiles += (range[j].y - range[j].x + height - 1) / height;
     }
-    before += n;
+    const uint32_t upto = wave_inclusive_scan_u32(tiles);
+    if (threadIdx.x % kWave == kWave - 1) wave_total[threadIdx.x / kWave] = upto;
+    __syncthreads();
+    before = upto - tiles;
+    *total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      before += w < threadIdx.x / kWave ? wave_total[w] : 0u;
+      *total += wave_total[w];
+    }
   }
-  __syncthreads();
-  return found;
-}
+  // index < total
+  __device__ __forceinline__ Tile find(uint32_t index) const {
+    uint32_t at = before;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; ++j) {
+      const uint32_t n = (range[j].y - range[j].x + height - 1) / height;
+      if (index >= at && index - at < n) {
+        const uint32_t first = range[j].x + (index - at) * height;
+        *found = Tile{threadIdx.x * per + j, first, range[j].y - first < height ? range[j].y : first + height};
+      }
+      at += n;
+    }
+    __syncthreads();
+    return *found;
+  }
+};
 
 uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
   // every expert (and the rows behind the last) has at most one tile that is not full
@@ -66,84 +80,297 @@ uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
   return static_cast<uint64_t>(rows) / height + (partly < rows ? partly : rows);
 }
 
-// out = rows @ weight[expert], tiles of 64 x 64, 16 of the inner dimension at a time in LDS, 4 x 4 results to a thread.
-constexpr uint32_t kTile = 64, kStep = 16;
+// ---- tiles --------------------------------------------------------------------------------------------------------
+// One product kernel body for the three products.  C[m][n] = sum over k of A[m][k] B[n][k], tiles of BM x BN, kDepth (128 bytes
+// of a row) of k at a time through two buffers in LDS.  An operand lies in memory with its k side by side ("along": rows of
+// tokens, out-major weights) or with its m or n side by side ("across": the others).
+//   along:  LDS holds [m][k], 128 bytes a row; a lane reads the 16 bytes of k that its matrix instruction takes.
+//   across: LDS holds [k][m]; 16-bit types are transposed by the LDS's transposing read (16 lanes read 4 rows of 16
+//           elements and get a column of 4 each), 32-bit ones are read one by one.
+// 16-byte pieces are placed so that the lanes of a read meet different banks (place()).
+template <typename T>
+struct Unit;  // the matrix instructions of a type: one piece of k (kPieceK elements) of 32 x 32 results
+template <>
+struct Unit<half_t> {
+  typedef half_t frag __attribute__((ext_vector_type(8)));
+  typedef float acc __attribute__((ext_vector_type(16)));
+  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Unit<bfloat_t> {
+  typedef bfloat_t frag __attribute__((ext_vector_type(8)));
+  typedef float acc __attribute__((ext_vector_type(16)));
+  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Unit<float> {
+  typedef float frag __attribute__((ext_vector_type(4)));
+  typedef float acc __attribute__((ext_vector_type(16)));
+  // (four steps of k = 2: the lower lanes hold k 0 to 3 of the piece, the upper 4 to 7; both operands alike)
+  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
 
-template <typename T, bool OUT_MAJOR>
-__global__ __launch_bounds__(kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
-                                                           const uint32_t *__restrict__ indptr, T *__restrict__ out,
-                                                           uint32_t n_rows, uint32_t experts, uint32_t inner, uint32_t cols) {
-  __shared__ float a[kStep][kTile + 1], b[kStep][kTile + 1];
-  const Tile tile = find_tile(indptr, experts, n_rows, kTile, blockIdx.y);
-  if (tile.expert == kNoTile) return;
-  const uint32_t col0 = blockIdx.x * kTile, ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float sum[4][4] = {};
-  if (tile.expert < experts) {
-    const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
-    for (uint32_t k0 = 0; k0 < inner; k0 += kStep) {
-      for (uint32_t i = threadIdx.x; i < kTile * kStep; i += kThreads) {
-        const uint32_t r = i / kStep, kk = i % kStep;
-        a[kk][r] = tile.first + r < tile.end && k0 + kk < inner
-                       ? static_cast<float>(rows[static_cast<size_t>(tile.first + r) * inner + k0 + kk]) : 0.f;
-        const uint32_t c = OUT_MAJOR ? i / kStep : i % kTile, kb = OUT_MAJOR ? i % kStep : i / kTile;
-        b[kb][c] = col0 + c < cols && k0 + kb < inner
-                       ? static_cast<float>(w[OUT_MAJOR ? static_cast<size_t>(col0 + c) * inner + k0 + kb
-                                                        : static_cast<size_t>(k0 + kb) * cols + col0 + c]) : 0.f;
+constexpr uint32_t kDepthBytes = 128;
+template <typename T>
+constexpr uint32_t kDepth = kDepthBytes / sizeof(T);
+
+// Where piece `piece` of row `row` lies, in pieces of 16 bytes.  along: rows of 8 pieces.  across: rows of WIDTH elements; the
+// 16-bit transposing read takes two neighbouring pieces of four rows.
+template <typename T, bool ACROSS, uint32_t WIDTH>
+__device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+  if (!ACROSS) return row * 8u + (piece ^ ((row >> 1) & 7u));
+  constexpr uint32_t kPieces = WIDTH / Piece<T>::kElems;
+  if (sizeof(T) == 4) return row * kPieces + piece;
+  constexpr uint32_t kPairs = kPieces / 2;  // pairs of pieces in a row: a power of two
+  constexpr uint32_t kSpread = kPairs >= 8 ? 2u : 1u;
+  return row * kPieces + (piece ^ ((((row & 3u) * kSpread) & (kPairs - 1u)) << 1));
+}
+
+// The piece of an operand that a thread brings: `first` .. `end`, the rows (m or n) that there are.
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS>
+struct Loader {
+  static constexpr uint32_t kElems = Piece<T>::kElems;
+  static constexpr uint32_t kPieces = WIDTH * kDepthBytes / 16 / THREADS;
+  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : 8u;
+  static_assert(WIDTH * kDepthBytes / 16 % THREADS == 0, "whole rounds");
+  typename Piece<T>::type held[kPieces];
+
+  // base: element (k = 0, first row) of the operand; `rows` of it are there, `stride` elements from one line to the next
+  __device__ __forceinline__ void load(const T *__restrict__ base, uint32_t rows, size_t stride, uint32_t k0, uint32_t depth) {
+#pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i) {
+      const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces, piece = at % kRowPieces;
+      held[i] = typename Piece<T>::type{};
+      if (ACROSS) {
+        if (k0 + line < depth && piece * kElems < rows) held[i] = load_piece<T>(base + (k0 + line) * stride, piece * kElems, rows);
+      } else {
+        if (line < rows && k0 + piece * kElems < depth) held[i] = load_piece<T>(base + line * stride, k0 + piece * kElems, depth);
       }
-      __syncthreads();
-#pragma unroll
-      for (uint32_t kk = 0; kk < kStep; ++kk)
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) sum[i][j] = fmaf(a[kk][ty * 4 + i], b[kk][tx + 16 * j], sum[i][j]);
-      __syncthreads();
     }
   }
+  __device__ __forceinline__ void store(T *lds) const {
 #pragma unroll
-  for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t r = tile.first + ty * 4 + i, c = col0 + tx + 16 * j;
-      if (r < tile.end && c < cols) out[static_cast<size_t>(r) * cols + c] = static_cast<T>(sum[i][j]);
+    for (uint32_t i = 0; i < kPieces; ++i) {
+      const uint32_t at = threadIdx.x + i * THREADS;
+      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH>(at / kRowPieces, at % kRowPieces)] =
+          __builtin_bit_cast(float4, held[i]);
     }
+  }
+};
+
+// What a lane gives the matrix unit: of row `row0` + lane % 32, piece 2 * step + lane / 32 of k.
+template <typename T, bool ACROSS, uint32_t WIDTH>
+__device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_t row0, uint32_t step) {
+  typedef typename Unit<T>::frag frag;
+  const uint32_t lane = threadIdx.x % kWave;
+  if constexpr (!ACROSS) {
+    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH>(row0 + lane % 32, 2 * step + lane / 32)]);
+  } else if constexpr (sizeof(T) == 4) {
+    frag f;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) f[j] = lds[(step * 8 + lane / 32 * 4 + j) * WIDTH + row0 + lane % 32];
+    return f;
+  } else {
+    typedef short quad __attribute__((ext_vector_type(4)));
+    quad half[2];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t k = step * 16 + lane / 32 * 8 + j * 4 + lane % 16 / 4, col = row0 + lane % 32 / 16 * 16 + lane % 4 * 4;
+      const T *from = lds + place<T, true, WIDTH>(k, col / 8) * 8 + col % 8;
+      half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) quad *)from);
+    }
+    return __builtin_bit_cast(frag, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// Shape of a tile: BM x BN results, WM x WN waves.
+template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_>
+struct Shape {
+  static constexpr uint32_t BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * kWave;
+  static constexpr uint32_t kFragsM = BM / WM / 32, kFragsN = BN / WN / 32;
+};
+template <typename T, typename S>
+constexpr uint32_t kLdsBytes = 2 * (S::BM + S::BN) * kDepthBytes;
+
+// The tile's results to `out` (row-major, `stride` elements a row): `rows` x `cols` of it are there.
+template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
+__device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t rows, size_t a_stride, const T *__restrict__ b,
+                                             uint32_t cols, size_t b_stride, uint32_t depth, T *__restrict__ out,
+                                             size_t out_stride, float4 *lds) {
+  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = 4;
+  T *const buffer = reinterpret_cast<T *>(lds);  // A, B of one buffer, then of the other
+  const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
+  typename Unit<T>::acc sum[S::kFragsM][S::kFragsN] = {};
+  Loader<T, A_ACROSS, S::BM, S::kThreads> load_a;
+  Loader<T, B_ACROSS, S::BN, S::kThreads> load_b;
+  if (depth != 0) {
+    load_a.load(a, rows, a_stride, 0, depth);
+    load_b.load(b, cols, b_stride, 0, depth);
+    load_a.store(buffer);
+    load_b.store(buffer + kA);
+  }
+  __syncthreads();
+  uint32_t turn = 0;
+  for (uint32_t k0 = 0; k0 < depth; k0 += kDepth<T>, turn ^= 1u) {
+    const bool more = k0 + kDepth<T> < depth;
+    if (more) {
+      load_a.load(a, rows, a_stride, k0 + kDepth<T>, depth);
+      load_b.load(b, cols, b_stride, k0 + kDepth<T>, depth);
+    }
+    const T *const at = buffer + turn * (kA + kB);
+#pragma unroll
+    for (uint32_t step = 0; step < kSteps; ++step) {
+      typename Unit<T>::frag fa[S::kFragsM], fb[S::kFragsN];
+#pragma unroll
+      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM>(at, m0 + i * 32, step);
+#pragma unroll
+      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN>(at + kA, n0 + j * 32, step);
+#pragma unroll
+      for (uint32_t i = 0; i < S::kFragsM; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = Unit<T>::mul(fb[j], fa[i], sum[i][j]);
+    }
+    if (more) {
+      T *const to = buffer + (turn ^ 1u) * (kA + kB);
+      load_a.store(to);
+      load_b.store(to + kA);
+    }
+    __syncthreads();
+  }
+  // Results to memory by way of LDS, whole pieces of a row side by side: a lane holds, of row lane % 32, 4 neighbouring
+  // columns at a time.  In 32 bits the tile may take the buffers' room twice: half its rows at a time.
+  constexpr uint32_t kOutPieces = S::BN / Piece<T>::kElems + 1;  // (a piece more, against bank conflicts)
+  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > kLdsBytes<T, S> ? S::WM : 1u, kPart = S::BM / kParts;
+  static_assert(kPart * kOutPieces * 16 <= kLdsBytes<T, S>, "the results fit");
+  typedef T quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (uint32_t part = 0; part < kParts; ++part) {
+    if (part != 0) __syncthreads();
+    if (kParts == 1 || wave / S::WN == part) {
+#pragma unroll
+      for (uint32_t i = 0; i < S::kFragsM; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < S::kFragsN; ++j)
+#pragma unroll
+          for (uint32_t r = 0; r < 4; ++r) {
+            quad v;
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
+            const uint32_t row = m0 - part * kPart + i * 32 + lane % 32, col = n0 + j * 32 + r * 8 + lane / 32 * 4;
+            *reinterpret_cast<quad *>(buffer + row * kOutPieces * Piece<T>::kElems + col) = v;
+          }
+    }
+    __syncthreads();
+    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
+    for (uint32_t at = threadIdx.x; at < kPart * kRow; at += S::kThreads) {
+      const uint32_t row = at / kRow, piece = at % kRow;
+      if (part * kPart + row < rows && piece * Piece<T>::kElems < cols)
+        store_piece<T>(out + (part * kPart + row) * out_stride, piece * Piece<T>::kElems, cols,
+                       __builtin_bit_cast(typename Piece<T>::type, lds[row * kOutPieces + piece]));
+    }
+  }
+}
+
+// Which tile a workgroup takes: those of a run lie on one XCD (workgroups go round the eight), where they share an L2.
+__device__ __forceinline__ uint64_t tile_of(uint64_t block, uint64_t tiles) {
+  const uint64_t share = (tiles + 7) / 8;
+  const uint64_t index = block % 8 * share + block / 8;
+  return block / 8 < share && index < tiles ? index : ~0ull;
+}
+unsigned grid_of(uint64_t tiles) { return static_cast<unsigned>((tiles + 7) / 8 * 8); }
+
+template <typename T, bool OUT_MAJOR, typename S>
+__global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
+                                                              const uint32_t *__restrict__ indptr, T *__restrict__ out,
+                                                              uint32_t n_rows, uint32_t experts, uint32_t inner,
+                                                              uint32_t cols) {
+  extern __shared__ float4 lds[];
+  const uint32_t across = (cols + S::BN - 1) / S::BN;
+  uint32_t total;
+  TileFinder<S::kThreads> finder(indptr, experts, n_rows, S::BM, &total);
+  const uint64_t index = tile_of(blockIdx.x, static_cast<uint64_t>(total) * across);
+  if (index == ~0ull) return;
+  const Tile tile = finder.find(static_cast<uint32_t>(index / across));
+  const uint32_t col0 = static_cast<uint32_t>(index % across) * S::BN;
+  const uint32_t width = cols - col0 < S::BN ? cols - col0 : S::BN;
+  T *const to = out + static_cast<size_t>(tile.first) * cols + col0;
+  if (tile.expert >= experts) {  // rows behind the last expert's
+    typename Piece<T>::type zero{};
+    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
+    for (uint32_t at = threadIdx.x; at < (tile.end - tile.first) * kRow; at += S::kThreads)
+      if (at % kRow * Piece<T>::kElems < width)
+        store_piece<T>(to + static_cast<size_t>(at / kRow) * cols, at % kRow * Piece<T>::kElems, width, zero);
+    return;
+  }
+  const T *const a = rows + static_cast<size_t>(tile.first) * inner;
+  const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
+  tile_product<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0,
+                                        width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
 }
 
 // d_weight[expert] = left_e^T @ right_e over the expert's rows; (left, right) = (rows, ct), or (ct, rows) where the weight is
 // stored out-major.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
-                                                            const uint32_t *__restrict__ indptr, T *__restrict__ d_weight,
-                                                            uint32_t n_rows, uint32_t experts, uint32_t n_left, uint32_t n_right) {
-  __shared__ float a[kStep][kTile + 1], b[kStep][kTile + 1];
-  const uint32_t expert = blockIdx.z, p0 = blockIdx.y * kTile, q0 = blockIdx.x * kTile;
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
+                                                               const uint32_t *__restrict__ indptr, T *__restrict__ d_weight,
+                                                               uint32_t n_rows, uint32_t experts, uint32_t n_left,
+                                                               uint32_t n_right) {
+  extern __shared__ float4 lds[];
+  const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
+  const uint64_t index = tile_of(blockIdx.x, static_cast<uint64_t>(experts) * down * across);
+  if (index == ~0ull) return;
+  const uint32_t expert = static_cast<uint32_t>(index / (static_cast<uint64_t>(down) * across));
+  const uint32_t in = static_cast<uint32_t>(index % (static_cast<uint64_t>(down) * across));
+  const uint32_t p0 = in / across * S::BM, q0 = in % across * S::BN;
   const uint2 range = rows_of(indptr, expert, experts, n_rows);
-  const uint32_t ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float sum[4][4] = {};
-  for (uint32_t r0 = range.x; r0 < range.y; r0 += kStep) {
-    for (uint32_t i = threadIdx.x; i < kTile * kStep; i += kThreads) {
-      const uint32_t r = i / kTile, c = i % kTile;
-      const bool inside = r0 + r < range.y;
-      a[r][c] = inside && p0 + c < n_left ? static_cast<float>(left[static_cast<size_t>(r0 + r) * n_left + p0 + c]) : 0.f;
-      b[r][c] = inside && q0 + c < n_right ? static_cast<float>(right[static_cast<size_t>(r0 + r) * n_right + q0 + c]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t kk = 0; kk < kStep; ++kk)
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) sum[i][j] = fmaf(a[kk][ty * 4 + i], b[kk][tx + 16 * j], sum[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t p = p0 + ty * 4 + i, q = q0 + tx + 16 * j;
-      if (p < n_left && q < n_right)
-        d_weight[(static_cast<size_t>(expert) * n_left + p) * n_right + q] = static_cast<T>(sum[i][j]);
-    }
+  tile_product<T, true, true, S>(left + static_cast<size_t>(range.x) * n_left + p0, n_left - p0 < S::BM ? n_left - p0 : S::BM, n_left,
+                                 right + static_cast<size_t>(range.x) * n_right + q0,
+                                 n_right - q0 < S::BN ? n_right - q0 : S::BN, n_right, range.y - range.x,
+                                 d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0, n_right, lds);
+}
+
+bool refuse_grid(const char *target, uint64_t tiles) {
+  if (tiles < (1u << 22)) return false;  // (threads of a launch are counted in 32 bits)
+  set_error("%s: a product of %llu tiles is too large for one call", target, static_cast<unsigned long long>(tiles));
+  return true;
+}
+
+// More than 64 KB of LDS has to be asked for, once a kernel and device.
+template <typename K>
+bool allow_lds(const char *target, K kernel, uint32_t bytes) {
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(bytes));
+  if (e == hipSuccess) return true;
+  (void)hipGetLastError();
+  set_error("%s: %u bytes of LDS: %s", target, bytes, hipGetErrorString(e));
+  return false;
+}
+
+using Large = Shape<256, 256, 2, 4>;
+using Middle = Shape<128, 128, 2, 2>;
+using Small = Shape<64, 64, 2, 2>;
+
+template <typename T, typename S>
+void launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
+  const uint64_t tiles = most_tiles(d.rows, d.experts, S::BM) * div_up(d.out, S::BN);
+  if (refuse_grid(target, tiles)) return;
+  const auto launch = [&](auto *kernel) {
+    if (!allow_lds(target, kernel, kLdsBytes<T, S>)) return;
+    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream,
+                       static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
+                       static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
+                       d.out);
+    check_launch(target);
+  };
+  if (d.flags & BPL_EXPERT_OUT_MAJOR)
+    launch(product_kernel<T, true, S>);
+  else
+    launch(product_kernel<T, false, S>);
 }
 
 template <typename T>
@@ -151,17 +378,23 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
   bpl_expert_descriptor d;
   if (!unpack(target, opaque, opaque_len, &d) || !expert_limits(target, d)) return;
   if (d.rows == 0 || d.out == 0) return;
-  const uint64_t tiles = most_tiles(d.rows, d.experts, kTile);
-  const auto launch = [&](auto *kernel) {
-    hipLaunchKernelGGL(kernel, dim3(div_up(d.out, kTile), static_cast<unsigned>(tiles)), dim3(kThreads), 0, stream,
-                       static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
-                       static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
-                       d.out);
-  };
-  if (d.flags & BPL_EXPERT_OUT_MAJOR)
-    launch(product_kernel<T, true>);
+  const uint32_t mean = d.rows / d.experts;
+  if (sizeof(T) == 2 && mean >= 192)
+    launch_product<T, std::conditional_t<sizeof(T) == 2, Large, Middle>>(target, stream, d, buffers);
+  else if (mean >= 48)
+    launch_product<T, Middle>(target, stream, d, buffers);
   else
-    launch(product_kernel<T, false>);
+    launch_product<T, Small>(target, stream, d, buffers);
+}
+
+template <typename T, typename S>
+void launch_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
+                     uint32_t n_left, uint32_t n_right, void **buffers) {
+  const uint64_t tiles = static_cast<uint64_t>(d.experts) * div_up(n_left, S::BM) * div_up(n_right, S::BN);
+  if (refuse_grid(target, tiles) || !allow_lds(target, gradient_kernel<T, S>, kLdsBytes<T, S>)) return;
+  hipLaunchKernelGGL((gradient_kernel<T, S>), dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream,
+                     static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
+                     static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
   check_launch(target);
 }
 
@@ -172,11 +405,11 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   if (d.width == 0 || d.out == 0) return;
   const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
   const uint32_t n_left = out_major ? d.out : d.width, n_right = out_major ? d.width : d.out;
-  hipLaunchKernelGGL(gradient_kernel<T>, dim3(div_up(n_right, kTile), div_up(n_left, kTile), d.experts), dim3(kThreads), 0,
-                     stream, static_cast<const T *>(buffers[out_major ? 1 : 0]),
-                     static_cast<const T *>(buffers[out_major ? 0 : 1]), static_cast<const uint32_t *>(buffers[2]),
-                     static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
-  check_launch(target);
+  const void *const left = buffers[out_major ? 1 : 0], *const right = buffers[out_major ? 0 : 1];
+  if (sizeof(T) == 2 && static_cast<uint64_t>(d.experts) * div_up(n_left, 256) * div_up(n_right, 256) >= 256)
+    launch_gradient<T, std::conditional_t<sizeof(T) == 2, Large, Middle>>(target, stream, d, left, right, n_left, n_right, buffers);
+  else
+    launch_gradient<T, Middle>(target, stream, d, left, right, n_left, n_right, buffers);
 }
 
 }  // namespace
