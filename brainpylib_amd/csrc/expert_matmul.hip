@@ -10,6 +10,18 @@ namespace {
 
 using namespace bpl;
 
+// A value that all lanes of a wave have, as the scalar that it is.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+}
+
+template <typename T>
+__device__ __forceinline__ const T *uniform(const T *p) {
+  const auto v = reinterpret_cast<uintptr_t>(p);
+  const uint32_t low = uniform(static_cast<uint32_t>(v)), high = uniform(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const T *>(static_cast<uintptr_t>(high) << 32 | low);
+}
+
 // The rows of expert e, whatever indptr says within the array; e == experts: the rows behind the last.
 __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, uint32_t e, uint32_t experts, uint32_t rows) {
   uint32_t from = e == 0 ? 0u : indptr[e], to = e < experts ? indptr[e + 1] : rows;
@@ -18,6 +30,7 @@ __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, ui
   return make_uint2(from, to > from ? to : from);
 }
 
+constexpr uint32_t kNoTile = 0xffffffffu;
 struct Tile {
   uint32_t expert, first, end;  // the rows of the tile: [first, end)
 };
@@ -56,6 +69,7 @@ struct TileFinder {
       before += w < threadIdx.x / kWave ? wave_total[w] : 0u;
       *total += wave_total[w];
     }
+    *total = uniform(*total);
   }
   // index < total
   __device__ __forceinline__ Tile find(uint32_t index) const {
@@ -70,7 +84,8 @@ struct TileFinder {
       at += n;
     }
     __syncthreads();
-    return *found;
+    // (the same for all lanes, and the compiler is to know it: addresses of the loads are scalars)
+    return Tile{uniform(found->expert), uniform(found->first), uniform(found->end)};
   }
 };
 
@@ -196,6 +211,50 @@ struct Shape {
 template <typename T, typename S>
 constexpr uint32_t kLdsBytes = 2 * (S::BM + S::BN) * kDepthBytes;
 
+template <typename T, typename S>
+using Sums = typename Unit<T>::acc[S::kFragsM][S::kFragsN];
+
+// The tile's results to memory by way of LDS (which nothing else uses any more), whole pieces of a row side by side: a lane
+// holds, of row lane % 32, 4 neighbouring columns at a time.  Where the tile takes more than the buffers' room, a row of
+// waves at a time.
+template <typename T, typename S>
+__device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t rows, uint32_t cols, T *__restrict__ out,
+                                           size_t out_stride, float4 *lds) {
+  T *const buffer = reinterpret_cast<T *>(lds);
+  const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
+  constexpr uint32_t kOutPieces = S::BN / Piece<T>::kElems + 1;  // (a piece more, against bank conflicts)
+  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > kLdsBytes<T, S> ? S::WM : 1u, kPart = S::BM / kParts;
+  static_assert(kPart * kOutPieces * 16 <= kLdsBytes<T, S>, "the results fit");
+  typedef T quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (uint32_t part = 0; part < kParts; ++part) {
+    if (part != 0) __syncthreads();
+    if (kParts == 1 || wave / S::WN == part) {
+#pragma unroll
+      for (uint32_t i = 0; i < S::kFragsM; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < S::kFragsN; ++j)
+#pragma unroll
+          for (uint32_t r = 0; r < 4; ++r) {
+            quad v;
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
+            const uint32_t row = m0 - part * kPart + i * 32 + lane % 32, col = n0 + j * 32 + r * 8 + lane / 32 * 4;
+            *reinterpret_cast<quad *>(buffer + row * kOutPieces * Piece<T>::kElems + col) = v;
+          }
+    }
+    __syncthreads();
+    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
+    for (uint32_t at = threadIdx.x; at < kPart * kRow; at += S::kThreads) {
+      const uint32_t row = at / kRow, piece = at % kRow;
+      if (part * kPart + row < rows && piece * Piece<T>::kElems < cols)
+        store_piece<T>(out + (part * kPart + row) * out_stride, piece * Piece<T>::kElems, cols,
+                       __builtin_bit_cast(typename Piece<T>::type, lds[row * kOutPieces + piece]));
+    }
+  }
+}
+
 // The tile's results to `out` (row-major, `stride` elements a row): `rows` x `cols` of it are there.
 template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
 __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t rows, size_t a_stride, const T *__restrict__ b,
@@ -203,7 +262,7 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
                                              size_t out_stride, float4 *lds) {
   constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = 4;
   T *const buffer = reinterpret_cast<T *>(lds);  // A, B of one buffer, then of the other
-  const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const uint32_t wave = threadIdx.x / kWave;
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
   typename Unit<T>::acc sum[S::kFragsM][S::kFragsN] = {};
   Loader<T, A_ACROSS, S::BM, S::kThreads> load_a;
@@ -242,49 +301,160 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     }
     __syncthreads();
   }
-  // Results to memory by way of LDS, whole pieces of a row side by side: a lane holds, of row lane % 32, 4 neighbouring
-  // columns at a time.  In 32 bits the tile may take the buffers' room twice: half its rows at a time.
-  constexpr uint32_t kOutPieces = S::BN / Piece<T>::kElems + 1;  // (a piece more, against bank conflicts)
-  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > kLdsBytes<T, S> ? S::WM : 1u, kPart = S::BM / kParts;
-  static_assert(kPart * kOutPieces * 16 <= kLdsBytes<T, S>, "the results fit");
-  typedef T quad __attribute__((ext_vector_type(4)));
+  store_tile<T, S>(sum, rows, cols, out, out_stride, lds);
+}
+
+// ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
+// For operands whose lines begin at multiples of 16 bytes.  A buffer is filled while the other is worked on: the fill of
+// tile t + 2 of k begins when every wave holds its last fragments of tile t, and is waited for a whole tile later, so one
+// barrier a tile is enough.  Fragments are read one step ahead, between the matrix instructions, which a single wave on a
+// SIMD keeps busy by itself.
+//
+// The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
+// counts its own, and waits that count more loads than it knows are longer, never shorter.
+__device__ __forceinline__ void load_to_lds(uint32_t lds_bytes, uint32_t offset, const void *base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS>
+struct DirectLoader {
+  static constexpr uint32_t kElems = Piece<T>::kElems;
+  static constexpr uint32_t kPieces = WIDTH * kDepthBytes / 16 / THREADS;
+  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : 8u;
+  static_assert(WIDTH * kDepthBytes / 16 % THREADS == 0, "whole rounds");
+  uint32_t offset[kPieces];  // bytes from the operand's element (k0, first row)
+
+  // Lane by lane the pieces of LDS are filled in order; place() is its own inverse, so what belongs at place p of a row is
+  // the row's piece place(p).
+  __device__ __forceinline__ DirectLoader(uint32_t rows, uint32_t stride) {
 #pragma unroll
-  for (uint32_t part = 0; part < kParts; ++part) {
-    if (part != 0) __syncthreads();
-    if (kParts == 1 || wave / S::WN == part) {
-#pragma unroll
-      for (uint32_t i = 0; i < S::kFragsM; ++i)
-#pragma unroll
-        for (uint32_t j = 0; j < S::kFragsN; ++j)
-#pragma unroll
-          for (uint32_t r = 0; r < 4; ++r) {
-            quad v;
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
-            const uint32_t row = m0 - part * kPart + i * 32 + lane % 32, col = n0 + j * 32 + r * 8 + lane / 32 * 4;
-            *reinterpret_cast<quad *>(buffer + row * kOutPieces * Piece<T>::kElems + col) = v;
-          }
-    }
-    __syncthreads();
-    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
-    for (uint32_t at = threadIdx.x; at < kPart * kRow; at += S::kThreads) {
-      const uint32_t row = at / kRow, piece = at % kRow;
-      if (part * kPart + row < rows && piece * Piece<T>::kElems < cols)
-        store_piece<T>(out + (part * kPart + row) * out_stride, piece * Piece<T>::kElems, cols,
-                       __builtin_bit_cast(typename Piece<T>::type, lds[row * kOutPieces + piece]));
+    for (uint32_t i = 0; i < kPieces; ++i) {
+      const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces;
+      const uint32_t piece = place<T, ACROSS, WIDTH>(line, at % kRowPieces) - line * kRowPieces;
+      if (ACROSS) {  // (columns beyond the last whole piece are not stored: any will do)
+        const uint32_t last = (rows - 1) / kElems;
+        offset[i] = (line * stride + (piece < last ? piece : last) * kElems) * static_cast<uint32_t>(sizeof(T));
+      } else {
+        offset[i] = ((line < rows ? line : rows - 1) * stride + piece * kElems) * static_cast<uint32_t>(sizeof(T));
+      }
     }
   }
+  __device__ __forceinline__ void load(uint32_t i, const T *base, uint32_t lds_bytes, uint32_t wave) const {
+    load_to_lds(lds_bytes + (i * THREADS + wave * kWave) * 16u, offset[i], base);
+  }
+};
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
+__device__ __forceinline__ void tile_product_direct(const T *__restrict__ a_, uint32_t rows, uint32_t a_stride,
+                                                    const T *__restrict__ b_, uint32_t cols, uint32_t b_stride, uint32_t depth,
+                                                    T *__restrict__ out, size_t out_stride, float4 *lds) {
+  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = 4;
+  constexpr uint32_t kBufferBytes = (S::BM + S::BN) * kDepthBytes;
+  const T *const a = uniform(a_), *const b = uniform(b_);
+  T *const buffer = reinterpret_cast<T *>(lds);
+  const uint32_t wave = uniform(threadIdx.x / kWave);
+  const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
+  const uint32_t lds_base = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float4 *)lds)));
+  typename Unit<T>::acc sum[S::kFragsM][S::kFragsN] = {};
+  const DirectLoader<T, A_ACROSS, S::BM, S::kThreads> load_a(rows, a_stride);
+  const DirectLoader<T, B_ACROSS, S::BN, S::kThreads> load_b(cols, b_stride);
+  constexpr uint32_t kLoadsA = decltype(load_a)::kPieces, kLoads = kLoadsA + decltype(load_b)::kPieces;
+  const uint32_t tiles = (depth + kDepth<T> - 1) / kDepth<T>;
+  const uint32_t whole = depth / kDepth<T>;  // the last one may be partial: that one goes by way of registers, with zeros
+  const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kDepth<T>;
+  const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kDepth<T>;
+
+  const auto load_one = [&](uint32_t t, uint32_t i) {
+    const uint32_t to = lds_base + (t & 1u) * kBufferBytes;
+    if (i < kLoadsA)
+      load_a.load(i, a + t * a_step, to, wave);
+    else
+      load_b.load(i - kLoadsA, b + t * b_step, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
+  };
+  const auto load_partial = [&](uint32_t t) {
+    Loader<T, A_ACROSS, S::BM, S::kThreads> la;
+    Loader<T, B_ACROSS, S::BN, S::kThreads> lb;
+    T *const to = buffer + (t & 1u) * (kA + kB);
+    la.load(a, rows, a_stride, t * kDepth<T>, depth);
+    la.store(to);
+    lb.load(b, cols, b_stride, t * kDepth<T>, depth);
+    lb.store(to + kA);
+  };
+  const auto fill = [&](uint32_t t) {
+    if (t < whole) {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) load_one(t, i);
+    } else if (t < tiles) {
+      load_partial(t);
+    }
+  };
+  const auto meet = [&] {
+    wait_for_loads();
+    __syncthreads();
+  };
+
+  fill(0);
+  meet();
+  fill(1);
+  typename Unit<T>::frag fa[2][S::kFragsM], fb[2][S::kFragsN];
+  constexpr uint32_t kReads = S::kFragsM + S::kFragsN, kMuls = S::kFragsM * S::kFragsN;
+  const auto read_one = [&](uint32_t t, uint32_t step, uint32_t i) {
+    const T *const at = buffer + (t & 1u) * (kA + kB);
+    // (in the order in which the products need them)
+    if (i == 0)
+      fb[step & 1u][0] = fragment<T, B_ACROSS, S::BN>(at + kA, n0, step);
+    else if (i <= S::kFragsM)
+      fa[step & 1u][i - 1] = fragment<T, A_ACROSS, S::BM>(at, m0 + (i - 1) * 32, step);
+    else
+      fb[step & 1u][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN>(at + kA, n0 + (i - S::kFragsM) * 32, step);
+  };
+  if (tiles != 0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
+  }
+  // READ: there is a tile t + 1; FILL: and a whole one t + 2
+  const auto work = [&](uint32_t t, auto READ, auto FILL) {
+#pragma unroll
+    for (uint32_t step = 0; step < kSteps; ++step) {
+      const bool last = step + 1 == kSteps;
+      if (last && READ.value) {
+        meet();  // every wave holds its last fragments of tile t; tile t + 1 is there
+        if (!FILL.value && t + 2 < tiles) load_partial(t + 2);
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < kMuls; ++q) {
+        const uint32_t i = q % S::kFragsM, j = q / S::kFragsM;
+        sum[i][j] = Unit<T>::mul(fb[step & 1u][j], fa[step & 1u][i], sum[i][j]);
+        if (!last || READ.value) {
+#pragma unroll
+          for (uint32_t r = q * kReads / kMuls; r < (q + 1) * kReads / kMuls; ++r) read_one(last ? t + 1 : t, (step + 1) % kSteps, r);
+        }
+        if (last && FILL.value) {
+#pragma unroll
+          for (uint32_t r = q * kLoads / kMuls; r < (q + 1) * kLoads / kMuls; ++r) load_one(t + 2, r);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  uint32_t t = 0;
+  for (; t + 2 < whole; ++t) work(t, std::true_type(), std::true_type());
+  for (; t + 1 < tiles; ++t) work(t, std::true_type(), std::false_type());
+  if (t < tiles) work(t, std::false_type(), std::false_type());
+  __syncthreads();
+  store_tile<T, S>(sum, rows, cols, out, out_stride, lds);
 }
 
 // Which tile a workgroup takes: those of a run lie on one XCD (workgroups go round the eight), where they share an L2.
-__device__ __forceinline__ uint64_t tile_of(uint64_t block, uint64_t tiles) {
-  const uint64_t share = (tiles + 7) / 8;
-  const uint64_t index = block % 8 * share + block / 8;
-  return block / 8 < share && index < tiles ? index : ~0ull;
+__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint64_t tiles) {
+  const uint32_t share = static_cast<uint32_t>((tiles + 7) / 8);
+  const uint32_t index = block % 8 * share + block / 8;
+  return block / 8 < share && index < tiles ? index : kNoTile;
 }
 unsigned grid_of(uint64_t tiles) { return static_cast<unsigned>((tiles + 7) / 8 * 8); }
 
-template <typename T, bool OUT_MAJOR, typename S>
+template <typename T, bool OUT_MAJOR, typename S, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
                                                               const uint32_t *__restrict__ indptr, T *__restrict__ out,
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
@@ -293,10 +463,10 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
   const uint32_t across = (cols + S::BN - 1) / S::BN;
   uint32_t total;
   TileFinder<S::kThreads> finder(indptr, experts, n_rows, S::BM, &total);
-  const uint64_t index = tile_of(blockIdx.x, static_cast<uint64_t>(total) * across);
-  if (index == ~0ull) return;
-  const Tile tile = finder.find(static_cast<uint32_t>(index / across));
-  const uint32_t col0 = static_cast<uint32_t>(index % across) * S::BN;
+  const uint32_t index = tile_of(blockIdx.x, static_cast<uint64_t>(total) * across);
+  if (index == kNoTile) return;
+  const Tile tile = finder.find(index / across);
+  const uint32_t col0 = uniform(index % across) * S::BN;
   const uint32_t width = cols - col0 < S::BN ? cols - col0 : S::BN;
   T *const to = out + static_cast<size_t>(tile.first) * cols + col0;
   if (tile.expert >= experts) {  // rows behind the last expert's
@@ -309,29 +479,35 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
   }
   const T *const a = rows + static_cast<size_t>(tile.first) * inner;
   const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
-  tile_product<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0,
-                                        width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
+  const T *const b = OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0;
+  if constexpr (DIRECT)
+    tile_product_direct<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
+  else
+    tile_product<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
 }
 
 // d_weight[expert] = left_e^T @ right_e over the expert's rows; (left, right) = (rows, ct), or (ct, rows) where the weight is
 // stored out-major.
-template <typename T, typename S>
+template <typename T, typename S, bool DIRECT>
 __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
                                                                const uint32_t *__restrict__ indptr, T *__restrict__ d_weight,
                                                                uint32_t n_rows, uint32_t experts, uint32_t n_left,
                                                                uint32_t n_right) {
   extern __shared__ float4 lds[];
   const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
-  const uint64_t index = tile_of(blockIdx.x, static_cast<uint64_t>(experts) * down * across);
-  if (index == ~0ull) return;
-  const uint32_t expert = static_cast<uint32_t>(index / (static_cast<uint64_t>(down) * across));
-  const uint32_t in = static_cast<uint32_t>(index % (static_cast<uint64_t>(down) * across));
-  const uint32_t p0 = in / across * S::BM, q0 = in % across * S::BN;
-  const uint2 range = rows_of(indptr, expert, experts, n_rows);
-  tile_product<T, true, true, S>(left + static_cast<size_t>(range.x) * n_left + p0, n_left - p0 < S::BM ? n_left - p0 : S::BM, n_left,
-                                 right + static_cast<size_t>(range.x) * n_right + q0,
-                                 n_right - q0 < S::BN ? n_right - q0 : S::BN, n_right, range.y - range.x,
-                                 d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0, n_right, lds);
+  const uint32_t index = tile_of(blockIdx.x, static_cast<uint64_t>(experts) * down * across);
+  if (index == kNoTile) return;
+  const uint32_t expert = uniform(index / (down * across)), in = index % (down * across);
+  const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
+  uint2 range = rows_of(indptr, expert, experts, n_rows);
+  range = make_uint2(uniform(range.x), uniform(range.y));
+  const T *const a = left + static_cast<size_t>(range.x) * n_left + p0, *const b = right + static_cast<size_t>(range.x) * n_right + q0;
+  const uint32_t high = n_left - p0 < S::BM ? n_left - p0 : S::BM, wide = n_right - q0 < S::BN ? n_right - q0 : S::BN;
+  T *const to = d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0;
+  if constexpr (DIRECT)
+    tile_product_direct<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
+  else
+    tile_product<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
 }
 
 bool refuse_grid(const char *target, uint64_t tiles) {
@@ -351,7 +527,13 @@ bool allow_lds(const char *target, K kernel, uint32_t bytes) {
   return false;
 }
 
-using Large = Shape<256, 256, 2, 4>;
+// Loads that go straight to LDS need lines at multiples of 16 bytes, and offsets within a tile in 32 bits.
+template <typename T>
+bool whole_pieces(const void *p, uint32_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % Piece<T>::kElems == 0 && stride < (1u << 20);
+}
+
+using Large = Shape<256, 256, 2, 2>;
 using Middle = Shape<128, 128, 2, 2>;
 using Small = Shape<64, 64, 2, 2>;
 
@@ -367,10 +549,20 @@ void launch_product(const char *target, hipStream_t stream, const bpl_expert_des
                        d.out);
     check_launch(target);
   };
-  if (d.flags & BPL_EXPERT_OUT_MAJOR)
-    launch(product_kernel<T, true, S>);
+  const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
+  if constexpr (sizeof(T) == 2) {
+    if (whole_pieces<T>(buffers[0], d.width) && whole_pieces<T>(buffers[1], out_major ? d.width : d.out)) {
+      if (out_major)
+        launch(product_kernel<T, true, S, true>);
+      else
+        launch(product_kernel<T, false, S, true>);
+      return;
+    }
+  }
+  if (out_major)
+    launch(product_kernel<T, true, S, false>);
   else
-    launch(product_kernel<T, false, S>);
+    launch(product_kernel<T, false, S, false>);
 }
 
 template <typename T>
@@ -391,11 +583,21 @@ template <typename T, typename S>
 void launch_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
                      uint32_t n_left, uint32_t n_right, void **buffers) {
   const uint64_t tiles = static_cast<uint64_t>(d.experts) * div_up(n_left, S::BM) * div_up(n_right, S::BN);
-  if (refuse_grid(target, tiles) || !allow_lds(target, gradient_kernel<T, S>, kLdsBytes<T, S>)) return;
-  hipLaunchKernelGGL((gradient_kernel<T, S>), dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream,
-                     static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
-                     static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
-  check_launch(target);
+  if (refuse_grid(target, tiles)) return;
+  const auto launch = [&](auto *kernel) {
+    if (!allow_lds(target, kernel, kLdsBytes<T, S>)) return;
+    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream, static_cast<const T *>(left),
+                       static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
+                       static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
+    check_launch(target);
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right)) {
+      launch(gradient_kernel<T, S, true>);
+      return;
+    }
+  }
+  launch(gradient_kernel<T, S, false>);
 }
 
 template <typename T>
