@@ -133,11 +133,11 @@ constexpr uint32_t kDepthBytes = 128;
 template <typename T>
 constexpr uint32_t kDepth = kDepthBytes / sizeof(T);
 
-// Where piece `piece` of row `row` lies, in pieces of 16 bytes.  along: rows of 8 pieces.  across: rows of WIDTH elements; the
+// Where piece `piece` of row `row` lies, in pieces of 16 bytes.  along: rows of DEPTH (4 or 8) pieces.  across: rows of WIDTH elements; the
 // 16-bit transposing read takes two neighbouring pieces of four rows.
-template <typename T, bool ACROSS, uint32_t WIDTH>
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH>
 __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
-  if (!ACROSS) return row * 8u + (piece ^ ((row >> 1) & 7u));
+  if (!ACROSS) return row * DEPTH + (piece ^ ((row / (16 / DEPTH)) & (DEPTH - 1u)));
   constexpr uint32_t kPieces = WIDTH / Piece<T>::kElems;
   if (sizeof(T) == 4) return row * kPieces + piece;
   constexpr uint32_t kPairs = kPieces / 2;  // pairs of pieces in a row: a power of two
@@ -171,19 +171,19 @@ struct Loader {
 #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
       const uint32_t at = threadIdx.x + i * THREADS;
-      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH>(at / kRowPieces, at % kRowPieces)] =
+      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH, 8>(at / kRowPieces, at % kRowPieces)] =
           __builtin_bit_cast(float4, held[i]);
     }
   }
 };
 
 // What a lane gives the matrix unit: of row `row0` + lane % 32, piece 2 * step + lane / 32 of k.
-template <typename T, bool ACROSS, uint32_t WIDTH>
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH>
 __device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_t row0, uint32_t step) {
   typedef typename Unit<T>::frag frag;
   const uint32_t lane = threadIdx.x % kWave;
   if constexpr (!ACROSS) {
-    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH>(row0 + lane % 32, 2 * step + lane / 32)]);
+    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH, DEPTH>(row0 + lane % 32, 2 * step + lane / 32)]);
   } else if constexpr (sizeof(T) == 4) {
     frag f;
 #pragma unroll
@@ -195,21 +195,22 @@ __device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) {
       const uint32_t k = step * 16 + lane / 32 * 8 + j * 4 + lane % 16 / 4, col = row0 + lane % 32 / 16 * 16 + lane % 4 * 4;
-      const T *from = lds + place<T, true, WIDTH>(k, col / 8) * 8 + col % 8;
+      const T *from = lds + place<T, true, WIDTH, DEPTH>(k, col / 8) * 8 + col % 8;
       half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) quad *)from);
     }
     return __builtin_bit_cast(frag, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
 }
 
-// Shape of a tile: BM x BN results, WM x WN waves.
-template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_>
+// Shape of a tile: BM x BN results, WM x WN waves; kStages: of the ring of loads that go straight to LDS, 0: staged through
+// registers into two buffers.
+template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t STAGES>
 struct Shape {
+  static constexpr uint32_t kStages = STAGES;
+  static constexpr uint32_t kLdsBytes = (BM_ + BN_) * (STAGES != 0 ? STAGES * 64u : 2u * kDepthBytes);
   static constexpr uint32_t BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * kWave;
   static constexpr uint32_t kFragsM = BM / WM / 32, kFragsN = BN / WN / 32;
 };
-template <typename T, typename S>
-constexpr uint32_t kLdsBytes = 2 * (S::BM + S::BN) * kDepthBytes;
 
 template <typename T, typename S>
 using Sums = typename Unit<T>::acc[S::kFragsM][S::kFragsN];
@@ -224,8 +225,8 @@ __device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t rows,
   const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
   constexpr uint32_t kOutPieces = S::BN / Piece<T>::kElems + 1;  // (a piece more, against bank conflicts)
-  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > kLdsBytes<T, S> ? S::WM : 1u, kPart = S::BM / kParts;
-  static_assert(kPart * kOutPieces * 16 <= kLdsBytes<T, S>, "the results fit");
+  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > S::kLdsBytes ? S::WM : 1u, kPart = S::BM / kParts;
+  static_assert(kPart * kOutPieces * 16 <= S::kLdsBytes, "the results fit");
   typedef T quad __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (uint32_t part = 0; part < kParts; ++part) {
@@ -286,9 +287,9 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     for (uint32_t step = 0; step < kSteps; ++step) {
       typename Unit<T>::frag fa[S::kFragsM], fb[S::kFragsN];
 #pragma unroll
-      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM>(at, m0 + i * 32, step);
+      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM, 8>(at, m0 + i * 32, step);
 #pragma unroll
-      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN>(at + kA, n0 + j * 32, step);
+      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN, 8>(at + kA, n0 + j * 32, step);
 #pragma unroll
       for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
@@ -305,24 +306,33 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
 }
 
 // ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
-// For operands whose lines begin at multiples of 16 bytes.  A buffer is filled while the other is worked on: the fill of
-// tile t + 2 of k begins when every wave holds its last fragments of tile t, and is waited for a whole tile later, so one
-// barrier a tile is enough.  Fragments are read one step ahead, between the matrix instructions, which a single wave on a
-// SIMD keeps busy by itself.
+// For operands whose lines begin at multiples of 16 bytes.  LDS holds a ring of S::kStages stages, 64 bytes of a row of k each.
+// Stage t is worked on while stage t + kStages - 1 is filled, into the place of t - 1; a wave waits for its own loads of
+// stage t + 1 with those of the later ones under way, then for the other waves: one barrier a stage.  A load and a read of
+// the next step's fragment go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a
+// SIMD may have no other.
 //
 // The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
 // counts its own, and waits that count more loads than it knows are longer, never shorter.
+constexpr uint32_t kStageDepth = 4;  // pieces of 16 bytes
+template <typename T>
+constexpr uint32_t kStageK = kStageDepth * Piece<T>::kElems;
+
 __device__ __forceinline__ void load_to_lds(uint32_t lds_bytes, uint32_t offset, const void *base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
 }
-__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <uint32_t UNDER_WAY>
+__device__ __forceinline__ void wait_for_loads() {
+  static_assert(UNDER_WAY < 64, "what the counter holds");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(UNDER_WAY) : "memory");
+}
 
 template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS>
 struct DirectLoader {
   static constexpr uint32_t kElems = Piece<T>::kElems;
-  static constexpr uint32_t kPieces = WIDTH * kDepthBytes / 16 / THREADS;
-  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : 8u;
-  static_assert(WIDTH * kDepthBytes / 16 % THREADS == 0, "whole rounds");
+  static constexpr uint32_t kPieces = WIDTH * kStageDepth / THREADS;
+  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : kStageDepth;
+  static_assert(WIDTH * kStageDepth % THREADS == 0, "whole rounds");
   uint32_t offset[kPieces];  // bytes from the operand's element (k0, first row)
 
   // Lane by lane the pieces of LDS are filled in order; place() is its own inverse, so what belongs at place p of a row is
@@ -331,7 +341,7 @@ struct DirectLoader {
 #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
       const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces;
-      const uint32_t piece = place<T, ACROSS, WIDTH>(line, at % kRowPieces) - line * kRowPieces;
+      const uint32_t piece = place<T, ACROSS, WIDTH, kStageDepth>(line, at % kRowPieces) - line * kRowPieces;
       if (ACROSS) {  // (columns beyond the last whole piece are not stored: any will do)
         const uint32_t last = (rows - 1) / kElems;
         offset[i] = (line * stride + (piece < last ? piece : last) * kElems) * static_cast<uint32_t>(sizeof(T));
@@ -343,105 +353,120 @@ struct DirectLoader {
   __device__ __forceinline__ void load(uint32_t i, const T *base, uint32_t lds_bytes, uint32_t wave) const {
     load_to_lds(lds_bytes + (i * THREADS + wave * kWave) * 16u, offset[i], base);
   }
+  // The last stage, of which only `depth` of k are there: by way of registers, with zeros behind.
+  static __device__ __forceinline__ void load_partial(const T *__restrict__ base, uint32_t rows, size_t stride, uint32_t depth, T *lds) {
+#pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i) {
+      const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces, piece = at % kRowPieces;
+      typename Piece<T>::type v{};
+      if (ACROSS) {
+        if (line < depth && piece * kElems < rows) v = load_piece<T>(base + line * stride, piece * kElems, rows);
+      } else {
+        if (line < rows && piece * kElems < depth) v = load_piece<T>(base + line * stride, piece * kElems, depth);
+      }
+      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH, kStageDepth>(line, piece)] = __builtin_bit_cast(float4, v);
+    }
+  }
 };
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
 __device__ __forceinline__ void tile_product_direct(const T *__restrict__ a_, uint32_t rows, uint32_t a_stride,
                                                     const T *__restrict__ b_, uint32_t cols, uint32_t b_stride, uint32_t depth,
                                                     T *__restrict__ out, size_t out_stride, float4 *lds) {
-  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = 4;
-  constexpr uint32_t kBufferBytes = (S::BM + S::BN) * kDepthBytes;
+  constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = kStageDepth / 2, kRing = S::kStages;
+  constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
+  static_assert((kRing & (kRing - 1)) == 0 && kRing >= 4, "a power of two");
   const T *const a = uniform(a_), *const b = uniform(b_);
   T *const buffer = reinterpret_cast<T *>(lds);
   const uint32_t wave = uniform(threadIdx.x / kWave);
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
   const uint32_t lds_base = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float4 *)lds)));
-  typename Unit<T>::acc sum[S::kFragsM][S::kFragsN] = {};
-  const DirectLoader<T, A_ACROSS, S::BM, S::kThreads> load_a(rows, a_stride);
-  const DirectLoader<T, B_ACROSS, S::BN, S::kThreads> load_b(cols, b_stride);
-  constexpr uint32_t kLoadsA = decltype(load_a)::kPieces, kLoads = kLoadsA + decltype(load_b)::kPieces;
-  const uint32_t tiles = (depth + kDepth<T> - 1) / kDepth<T>;
-  const uint32_t whole = depth / kDepth<T>;  // the last one may be partial: that one goes by way of registers, with zeros
-  const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kDepth<T>;
-  const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kDepth<T>;
+  Sums<T, S> sum = {};
+  typedef DirectLoader<T, A_ACROSS, S::BM, S::kThreads> LoaderA;
+  typedef DirectLoader<T, B_ACROSS, S::BN, S::kThreads> LoaderB;
+  const LoaderA load_a(rows, a_stride);
+  const LoaderB load_b(cols, b_stride);
+  constexpr uint32_t kLoads = LoaderA::kPieces + LoaderB::kPieces;
+  const uint32_t whole = depth / kStageK<T>, stages = (depth + kStageK<T> - 1) / kStageK<T>;
+  const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kStageK<T>;
+  const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
 
   const auto load_one = [&](uint32_t t, uint32_t i) {
-    const uint32_t to = lds_base + (t & 1u) * kBufferBytes;
-    if (i < kLoadsA)
+    const uint32_t to = lds_base + (t & (kRing - 1)) * kStageBytes;
+    if (i < LoaderA::kPieces)
       load_a.load(i, a + t * a_step, to, wave);
     else
-      load_b.load(i - kLoadsA, b + t * b_step, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
+      load_b.load(i - LoaderA::kPieces, b + t * b_step, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
   };
-  const auto load_partial = [&](uint32_t t) {
-    Loader<T, A_ACROSS, S::BM, S::kThreads> la;
-    Loader<T, B_ACROSS, S::BN, S::kThreads> lb;
-    T *const to = buffer + (t & 1u) * (kA + kB);
-    la.load(a, rows, a_stride, t * kDepth<T>, depth);
-    la.store(to);
-    lb.load(b, cols, b_stride, t * kDepth<T>, depth);
-    lb.store(to + kA);
-  };
-  const auto fill = [&](uint32_t t) {
+  const auto fill_rest = [&](uint32_t t) {  // a stage that may be partial, or none
+    T *const to = buffer + (t & (kRing - 1)) * (kA + kB);
     if (t < whole) {
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) load_one(t, i);
-    } else if (t < tiles) {
-      load_partial(t);
+    } else if (t < stages) {
+      LoaderA::load_partial(a + t * a_step, rows, a_stride, depth - t * kStageK<T>, to);
+      LoaderB::load_partial(b + t * b_step, cols, b_stride, depth - t * kStageK<T>, to + kA);
     }
   };
-  const auto meet = [&] {
-    wait_for_loads();
-    __syncthreads();
-  };
 
-  fill(0);
-  meet();
-  fill(1);
   typename Unit<T>::frag fa[2][S::kFragsM], fb[2][S::kFragsN];
   constexpr uint32_t kReads = S::kFragsM + S::kFragsN, kMuls = S::kFragsM * S::kFragsN;
   const auto read_one = [&](uint32_t t, uint32_t step, uint32_t i) {
-    const T *const at = buffer + (t & 1u) * (kA + kB);
+    const T *const at = buffer + (t & (kRing - 1)) * (kA + kB);
     // (in the order in which the products need them)
     if (i == 0)
-      fb[step & 1u][0] = fragment<T, B_ACROSS, S::BN>(at + kA, n0, step);
+      fb[step & 1u][0] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0, step);
     else if (i <= S::kFragsM)
-      fa[step & 1u][i - 1] = fragment<T, A_ACROSS, S::BM>(at, m0 + (i - 1) * 32, step);
+      fa[step & 1u][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth>(at, m0 + (i - 1) * 32, step);
     else
-      fb[step & 1u][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN>(at + kA, n0 + (i - S::kFragsM) * 32, step);
+      fb[step & 1u][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0 + (i - S::kFragsM) * 32, step);
   };
-  if (tiles != 0) {
-#pragma unroll
-    for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
-  }
-  // READ: there is a tile t + 1; FILL: and a whole one t + 2
-  const auto work = [&](uint32_t t, auto READ, auto FILL) {
+  // NEXT: there is a stage t + 1; FILL: and a whole one t + kRing - 1
+  const auto work = [&](uint32_t t, auto NEXT, auto FILL) {
 #pragma unroll
     for (uint32_t step = 0; step < kSteps; ++step) {
       const bool last = step + 1 == kSteps;
-      if (last && READ.value) {
-        meet();  // every wave holds its last fragments of tile t; tile t + 1 is there
-        if (!FILL.value && t + 2 < tiles) load_partial(t + 2);
+      if (last && NEXT.value) {  // stage t + 1 is there, and every wave holds its last fragments of stage t
+        wait_for_loads<FILL.value ? (kRing - 3) * kLoads + kLoads * (kSteps - 1) / kSteps : 0>();
+        __syncthreads();
       }
 #pragma unroll
       for (uint32_t q = 0; q < kMuls; ++q) {
         const uint32_t i = q % S::kFragsM, j = q / S::kFragsM;
         sum[i][j] = Unit<T>::mul(fb[step & 1u][j], fa[step & 1u][i], sum[i][j]);
-        if (!last || READ.value) {
+        if (!last || NEXT.value) {
 #pragma unroll
           for (uint32_t r = q * kReads / kMuls; r < (q + 1) * kReads / kMuls; ++r) read_one(last ? t + 1 : t, (step + 1) % kSteps, r);
         }
-        if (last && FILL.value) {
+        if (FILL.value) {
+          constexpr uint32_t kShare = kLoads / kSteps;
+          static_assert(kLoads % kSteps == 0, "an equal share to a step");
 #pragma unroll
-          for (uint32_t r = q * kLoads / kMuls; r < (q + 1) * kLoads / kMuls; ++r) load_one(t + 2, r);
+          for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r) load_one(t + kRing - 1, step * kShare + r);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
+
+#pragma unroll
+  for (uint32_t t = 0; t + 1 < kRing; ++t) fill_rest(t);
+  if (whole >= kRing - 1)
+    wait_for_loads<(kRing - 2) * kLoads>();
+  else
+    wait_for_loads<0>();
+  __syncthreads();
+  if (stages != 0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
+  }
   uint32_t t = 0;
-  for (; t + 2 < whole; ++t) work(t, std::true_type(), std::true_type());
-  for (; t + 1 < tiles; ++t) work(t, std::true_type(), std::false_type());
-  if (t < tiles) work(t, std::false_type(), std::false_type());
+  for (; t + kRing - 1 < whole; ++t) work(t, std::true_type(), std::true_type());
+  for (; t + 1 < stages; ++t) {
+    if (t + kRing - 1 == whole) fill_rest(t + kRing - 1);
+    work(t, std::true_type(), std::false_type());
+  }
+  if (t < stages) work(t, std::false_type(), std::false_type());
   __syncthreads();
   store_tile<T, S>(sum, rows, cols, out, out_stride, lds);
 }
@@ -454,7 +479,7 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t block, uint64_t tiles) {
 }
 unsigned grid_of(uint64_t tiles) { return static_cast<unsigned>((tiles + 7) / 8 * 8); }
 
-template <typename T, bool OUT_MAJOR, typename S, bool DIRECT>
+template <typename T, bool OUT_MAJOR, typename S>
 __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
                                                               const uint32_t *__restrict__ indptr, T *__restrict__ out,
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
@@ -480,7 +505,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
   const T *const a = rows + static_cast<size_t>(tile.first) * inner;
   const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
   const T *const b = OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0;
-  if constexpr (DIRECT)
+  if constexpr (S::kStages != 0)
     tile_product_direct<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
   else
     tile_product<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
@@ -488,23 +513,25 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
 
 // d_weight[expert] = left_e^T @ right_e over the expert's rows; (left, right) = (rows, ct), or (ct, rows) where the weight is
 // stored out-major.
-template <typename T, typename S, bool DIRECT>
+template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
                                                                const uint32_t *__restrict__ indptr, T *__restrict__ d_weight,
                                                                uint32_t n_rows, uint32_t experts, uint32_t n_left,
                                                                uint32_t n_right) {
   extern __shared__ float4 lds[];
   const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
-  const uint32_t index = tile_of(blockIdx.x, static_cast<uint64_t>(experts) * down * across);
-  if (index == kNoTile) return;
-  const uint32_t expert = uniform(index / (down * across)), in = index % (down * across);
+  // An eighth of every expert's tiles to an XCD, neighbouring ones: the XCDs' work is the same however long the experts are.
+  const uint32_t tiles = down * across, share = (tiles + 7) / 8;
+  const uint32_t expert = uniform(blockIdx.x / 8 / share);
+  const uint32_t in = (blockIdx.x + expert * tiles) % 8 * share + blockIdx.x / 8 % share;
+  if (in >= tiles) return;
   const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
   uint2 range = rows_of(indptr, expert, experts, n_rows);
   range = make_uint2(uniform(range.x), uniform(range.y));
   const T *const a = left + static_cast<size_t>(range.x) * n_left + p0, *const b = right + static_cast<size_t>(range.x) * n_right + q0;
   const uint32_t high = n_left - p0 < S::BM ? n_left - p0 : S::BM, wide = n_right - q0 < S::BN ? n_right - q0 : S::BN;
   T *const to = d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0;
-  if constexpr (DIRECT)
+  if constexpr (S::kStages != 0)
     tile_product_direct<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
   else
     tile_product<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
@@ -533,36 +560,46 @@ bool whole_pieces(const void *p, uint32_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % Piece<T>::kElems == 0 && stride < (1u << 20);
 }
 
-using Large = Shape<256, 256, 2, 2>;
-using Middle = Shape<128, 128, 2, 2>;
-using Small = Shape<64, 64, 2, 2>;
+// Shapes for operands in whole pieces, and for others
+struct Direct {
+  using Large = Shape<256, 256, 2, 2, 4>;
+  using Middle = Shape<128, 128, 2, 2, 4>;
+  using Small = Shape<64, 64, 2, 2, 8>;
+};
+struct Staged {
+  using Large = Shape<256, 256, 2, 4, 0>;
+  using Middle = Shape<128, 128, 2, 2, 0>;
+  using Small = Shape<64, 64, 2, 2, 0>;
+};
 
 template <typename T, typename S>
 void launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
   const uint64_t tiles = most_tiles(d.rows, d.experts, S::BM) * div_up(d.out, S::BN);
   if (refuse_grid(target, tiles)) return;
   const auto launch = [&](auto *kernel) {
-    if (!allow_lds(target, kernel, kLdsBytes<T, S>)) return;
-    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream,
+    if (!allow_lds(target, kernel, S::kLdsBytes)) return;
+    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), S::kLdsBytes, stream,
                        static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
                        static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
                        d.out);
     check_launch(target);
   };
-  const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
-  if constexpr (sizeof(T) == 2) {
-    if (whole_pieces<T>(buffers[0], d.width) && whole_pieces<T>(buffers[1], out_major ? d.width : d.out)) {
-      if (out_major)
-        launch(product_kernel<T, true, S, true>);
-      else
-        launch(product_kernel<T, false, S, true>);
-      return;
-    }
-  }
-  if (out_major)
-    launch(product_kernel<T, true, S, false>);
+  if (d.flags & BPL_EXPERT_OUT_MAJOR)
+    launch(product_kernel<T, true, S>);
   else
-    launch(product_kernel<T, false, S, false>);
+    launch(product_kernel<T, false, S>);
+}
+
+template <typename T, typename SHAPES>
+void choose_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
+  const uint32_t mean = d.rows / d.experts;
+  if constexpr (sizeof(T) == 2) {
+    if (mean >= 192) return launch_product<T, typename SHAPES::Large>(target, stream, d, buffers);
+  }
+  if (mean >= 48)
+    launch_product<T, typename SHAPES::Middle>(target, stream, d, buffers);
+  else
+    launch_product<T, typename SHAPES::Small>(target, stream, d, buffers);
 }
 
 template <typename T>
@@ -570,34 +607,32 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
   bpl_expert_descriptor d;
   if (!unpack(target, opaque, opaque_len, &d) || !expert_limits(target, d)) return;
   if (d.rows == 0 || d.out == 0) return;
-  const uint32_t mean = d.rows / d.experts;
-  if (sizeof(T) == 2 && mean >= 192)
-    launch_product<T, std::conditional_t<sizeof(T) == 2, Large, Middle>>(target, stream, d, buffers);
-  else if (mean >= 48)
-    launch_product<T, Middle>(target, stream, d, buffers);
+  const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
+  if (whole_pieces<T>(buffers[0], d.width) && whole_pieces<T>(buffers[1], out_major ? d.width : d.out))
+    choose_product<T, Direct>(target, stream, d, buffers);
   else
-    launch_product<T, Small>(target, stream, d, buffers);
+    choose_product<T, Staged>(target, stream, d, buffers);
 }
 
 template <typename T, typename S>
 void launch_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
                      uint32_t n_left, uint32_t n_right, void **buffers) {
-  const uint64_t tiles = static_cast<uint64_t>(d.experts) * div_up(n_left, S::BM) * div_up(n_right, S::BN);
-  if (refuse_grid(target, tiles)) return;
-  const auto launch = [&](auto *kernel) {
-    if (!allow_lds(target, kernel, kLdsBytes<T, S>)) return;
-    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), (kLdsBytes<T, S>), stream, static_cast<const T *>(left),
-                       static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
-                       static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
-    check_launch(target);
-  };
+  const uint64_t blocks = 8 * ((static_cast<uint64_t>(div_up(n_left, S::BM)) * div_up(n_right, S::BN) + 7) / 8) * d.experts;
+  if (refuse_grid(target, blocks) || !allow_lds(target, gradient_kernel<T, S>, S::kLdsBytes)) return;
+  hipLaunchKernelGGL((gradient_kernel<T, S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), S::kLdsBytes, stream,
+                     static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
+                     static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
+  check_launch(target);
+}
+
+template <typename T, typename SHAPES>
+void choose_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
+                     uint32_t n_left, uint32_t n_right, void **buffers) {
   if constexpr (sizeof(T) == 2) {
-    if (whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right)) {
-      launch(gradient_kernel<T, S, true>);
-      return;
-    }
+    if (static_cast<uint64_t>(d.experts) * div_up(n_left, 256) * div_up(n_right, 256) >= 256)
+      return launch_gradient<T, typename SHAPES::Large>(target, stream, d, left, right, n_left, n_right, buffers);
   }
-  launch(gradient_kernel<T, S, false>);
+  launch_gradient<T, typename SHAPES::Middle>(target, stream, d, left, right, n_left, n_right, buffers);
 }
 
 template <typename T>
@@ -608,10 +643,10 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
   const uint32_t n_left = out_major ? d.out : d.width, n_right = out_major ? d.width : d.out;
   const void *const left = buffers[out_major ? 1 : 0], *const right = buffers[out_major ? 0 : 1];
-  if (sizeof(T) == 2 && static_cast<uint64_t>(d.experts) * div_up(n_left, 256) * div_up(n_right, 256) >= 256)
-    launch_gradient<T, std::conditional_t<sizeof(T) == 2, Large, Middle>>(target, stream, d, left, right, n_left, n_right, buffers);
+  if (whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right))
+    choose_gradient<T, Direct>(target, stream, d, left, right, n_left, n_right, buffers);
   else
-    launch_gradient<T, Middle>(target, stream, d, left, right, n_left, n_right, buffers);
+    choose_gradient<T, Staged>(target, stream, d, left, right, n_left, n_right, buffers);
 }
 
 }  // namespace
