@@ -30,69 +30,70 @@ __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, ui
   return make_uint2(from, to > from ? to : from);
 }
 
-constexpr uint32_t kNoTile = 0xffffffffu;
+// The experts' rows and where their tiles of `height` rows begin, counted over the experts in their order: in LDS, built
+// by all threads of the workgroup (one barrier, and one for the caller to see it).
 struct Tile {
   uint32_t expert, first, end;  // the rows of the tile: [first, end)
 };
+struct TileTable {
+  uint32_t start[kMostExperts + 1];
+  uint2 range[kMostExperts];
+  uint32_t wave_total[16];
 
-// Tiles of `height` rows, counted over the experts in their order and the rows behind the last: all threads of the
-// workgroup scan the experts' numbers of tiles.
-template <uint32_t THREADS>
-struct TileFinder {
-  static constexpr uint32_t kPer = (kMostExperts + 1 + THREADS - 1) / THREADS, kWaves = THREADS / kWave;
-  uint2 range[kPer];
-  uint32_t before, per, height;
-
-  Tile *found;  // in LDS
-
-  __device__ __forceinline__ TileFinder(const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t rows, uint32_t height_,
-                                        uint32_t *total) : height(height_) {
-    __shared__ uint32_t wave_total[kWaves];
-    __shared__ Tile tile;
-    found = &tile;
-    if (threadIdx.x == 0) tile = Tile{experts, 0, 0};  // (nothing, should no thread find it)
-    per = (experts + 1 + THREADS - 1) / THREADS;
-    uint32_t tiles = 0;
+  // the number of tiles
+  template <uint32_t THREADS>
+  __device__ __forceinline__ uint32_t build(const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t rows, uint32_t height) {
+    constexpr uint32_t kPer = (kMostExperts + THREADS - 1) / THREADS, kWaves = THREADS / kWave;
+    const uint32_t per = (experts + THREADS - 1) / THREADS;
+    uint32_t own[kPer], tiles = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kPer; ++j) {
       const uint32_t e = threadIdx.x * per + j;
-      range[j] = j < per && e <= experts ? rows_of(indptr, e, experts, rows) : make_uint2(0, 0);
-      tiles += (range[j].y - range[j].x + height - 1) / height;
+      own[j] = 0;
+      if (j < per && e < experts) {
+        const uint2 r = rows_of(indptr, e, experts, rows);
+        range[e] = r;
+        own[j] = (r.y - r.x + height - 1) / height;
+      }
+      tiles += own[j];
     }
     const uint32_t upto = wave_inclusive_scan_u32(tiles);
     if (threadIdx.x % kWave == kWave - 1) wave_total[threadIdx.x / kWave] = upto;
     __syncthreads();
-    before = upto - tiles;
-    *total = 0;
+    uint32_t at = upto - tiles, total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; ++w) {
-      before += w < threadIdx.x / kWave ? wave_total[w] : 0u;
-      *total += wave_total[w];
+      at += w < threadIdx.x / kWave ? wave_total[w] : 0u;
+      total += wave_total[w];
     }
-    *total = uniform(*total);
-  }
-  // index < total
-  __device__ __forceinline__ Tile find(uint32_t index) const {
-    uint32_t at = before;
 #pragma unroll
     for (uint32_t j = 0; j < kPer; ++j) {
-      const uint32_t n = (range[j].y - range[j].x + height - 1) / height;
-      if (index >= at && index - at < n) {
-        const uint32_t first = range[j].x + (index - at) * height;
-        *found = Tile{threadIdx.x * per + j, first, range[j].y - first < height ? range[j].y : first + height};
-      }
-      at += n;
+      const uint32_t e = threadIdx.x * per + j;
+      if (j < per && e < experts) start[e] = at;
+      at += own[j];
     }
     __syncthreads();
-    // (the same for all lanes, and the compiler is to know it: addresses of the loads are scalars)
-    return Tile{uniform(found->expert), uniform(found->first), uniform(found->end)};
+    return uniform(total);
+  }
+
+  // index < the number of tiles; every wave by itself: the last expert that begins at or before it (those without tiles begin
+  // where the next one does), 64 places and then 16 at a time
+  __device__ __forceinline__ Tile find(uint32_t index, uint32_t experts, uint32_t height) const {
+    static_assert(kMostExperts <= 64 * 16, "two looks are enough");
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t coarse = __popcll(__ballot(lane * 16 < experts && start[lane * 16 < experts ? lane * 16 : 0] <= index));
+    const uint32_t e = (coarse - 1) * 16 + lane;
+    const uint32_t fine = __popcll(__ballot(lane < 16 && e < experts && start[e < experts ? e : 0] <= index));
+    const uint32_t expert = uniform((coarse - 1) * 16 + fine - 1);
+    const uint2 r = range[expert];
+    const uint32_t first = uniform(r.x) + (index - uniform(start[expert])) * height, end = uniform(r.y);
+    return Tile{expert, first, end - first < height ? end : first + height};
   }
 };
 
 uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
-  // every expert (and the rows behind the last) has at most one tile that is not full
-  const uint64_t partly = static_cast<uint64_t>(experts) + 1;
-  return static_cast<uint64_t>(rows) / height + (partly < rows ? partly : rows);
+  // every expert has at most one tile that is not full
+  return static_cast<uint64_t>(rows) / height + (experts < rows ? experts : rows);
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
@@ -215,43 +216,50 @@ struct Shape {
 template <typename T, typename S>
 using Sums = typename Unit<T>::acc[S::kFragsM][S::kFragsN];
 
-// The tile's results to memory by way of LDS (which nothing else uses any more), whole pieces of a row side by side: a lane
-// holds, of row lane % 32, 4 neighbouring columns at a time.  Where the tile takes more than the buffers' room, a row of
-// waves at a time.
-template <typename T, typename S>
-__device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t rows, uint32_t cols, T *__restrict__ out,
-                                           size_t out_stride, float4 *lds) {
-  T *const buffer = reinterpret_cast<T *>(lds);
-  const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
-  constexpr uint32_t kOutPieces = S::BN / Piece<T>::kElems + 1;  // (a piece more, against bank conflicts)
-  constexpr uint32_t kParts = S::BM * kOutPieces * 16 > S::kLdsBytes ? S::WM : 1u, kPart = S::BM / kParts;
-  static_assert(kPart * kOutPieces * 16 <= S::kLdsBytes, "the results fit");
+// A wave's results to memory by way of a piece of LDS of its own, so that whole pieces of a row go side by side: a lane holds,
+// of row lane % 32, 4 neighbouring columns at a time.  kRoom bytes hold 32 rows of so many of the wave's columns.
+template <typename T, typename S, uint32_t ROOM>
+__device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols,
+                                           T *__restrict__ out, size_t out_stride, T *room) {
+  constexpr uint32_t kElems = Piece<T>::kElems, kWide = S::BN / S::WN;
+  constexpr uint32_t kCols = ROOM / 32 / sizeof(T) < kWide ? ROOM / 32 / sizeof(T) : kWide, kRow = kCols / kElems;
+  static_assert(kCols % 8 == 0 && kWide % kCols == 0 && (kRow & (kRow - 1)) == 0, "whole groups of 8 columns");
   typedef T quad __attribute__((ext_vector_type(4)));
+  const uint32_t lane = threadIdx.x % kWave;
+  const bool whole = m0 + S::BM / S::WM <= rows && n0 + kWide <= cols;
 #pragma unroll
-  for (uint32_t part = 0; part < kParts; ++part) {
-    if (part != 0) __syncthreads();
-    if (kParts == 1 || wave / S::WN == part) {
+  for (uint32_t i = 0; i < S::kFragsM; ++i) {
 #pragma unroll
-      for (uint32_t i = 0; i < S::kFragsM; ++i)
+    for (uint32_t c0 = 0; c0 < kWide; c0 += kCols) {
 #pragma unroll
-        for (uint32_t j = 0; j < S::kFragsN; ++j)
+      for (uint32_t g = 0; g < kCols / 8; ++g) {
+        const uint32_t j = (c0 / 8 + g) / 4, r = (c0 / 8 + g) % 4;
+        quad v;
 #pragma unroll
-          for (uint32_t r = 0; r < 4; ++r) {
-            quad v;
+        for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
+        const uint32_t row = lane % 32, col = g * 8 + lane / 32 * 4;
+        // (pieces are placed by the row, against bank conflicts)
+        *reinterpret_cast<quad *>(room + (row * kRow + ((col / kElems) ^ (row & (kRow - 1)))) * kElems + col % kElems) = v;
+      }
+      // (a wave's LDS instructions are carried out in order)
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_sched_barrier(0);  // (or the compiler fetches the sums of all turns first, and spills them)
+      constexpr uint32_t kRows = kWave / kRow;  // that the lanes hold at a time
+      const uint32_t row0 = lane / kRow, piece = lane % kRow, n = n0 + c0 + piece * kElems;
+      const auto held = [&](uint32_t row) {
+        return __builtin_bit_cast(typename Piece<T>::type, reinterpret_cast<const float4 *>(room)[row * kRow + (piece ^ (row & (kRow - 1)))]);
+      };
+      T *const to = out + (m0 + i * 32 + row0) * out_stride + n;
+      if (whole) {
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
-            const uint32_t row = m0 - part * kPart + i * 32 + lane % 32, col = n0 + j * 32 + r * 8 + lane / 32 * 4;
-            *reinterpret_cast<quad *>(buffer + row * kOutPieces * Piece<T>::kElems + col) = v;
-          }
-    }
-    __syncthreads();
-    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
-    for (uint32_t at = threadIdx.x; at < kPart * kRow; at += S::kThreads) {
-      const uint32_t row = at / kRow, piece = at % kRow;
-      if (part * kPart + row < rows && piece * Piece<T>::kElems < cols)
-        store_piece<T>(out + (part * kPart + row) * out_stride, piece * Piece<T>::kElems, cols,
-                       __builtin_bit_cast(typename Piece<T>::type, lds[row * kOutPieces + piece]));
+        for (uint32_t p = 0; p < 32; p += kRows) *reinterpret_cast<typename Piece<T>::type *>(to + p * out_stride) = held(p + row0);
+      } else {
+#pragma unroll 1
+        for (uint32_t p = 0; p < 32; p += kRows)
+          if (m0 + i * 32 + p + row0 < rows && n < cols) store_piece<T>(to + p * out_stride - n, n, cols, held(p + row0));
+      }
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -302,15 +310,17 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     }
     __syncthreads();
   }
-  store_tile<T, S>(sum, rows, cols, out, out_stride, lds);
+  constexpr uint32_t kRoom = S::kLdsBytes / (S::WM * S::WN) >= 8192 ? 8192 : S::kLdsBytes / (S::WM * S::WN);
+  store_tile<T, S, kRoom>(sum, m0, n0, rows, cols, out, out_stride, buffer + wave * (kRoom / sizeof(T)));
 }
 
 // ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
-// For operands whose lines begin at multiples of 16 bytes.  LDS holds a ring of S::kStages stages, 64 bytes of a row of k each.
-// Stage t is worked on while stage t + kStages - 1 is filled, into the place of t - 1; a wave waits for its own loads of
-// stage t + 1 with those of the later ones under way, then for the other waves: one barrier a stage.  A load and a read of
-// the next step's fragment go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a
-// SIMD may have no other.
+// For operands whose lines begin at multiples of 16 bytes.  A workgroup takes one tile after the other, and their stages
+// (64 bytes of a row of k each) are one stream through a ring of S::kStages places in LDS: stage g is worked on while stage
+// g + kStages - 1, perhaps the next tile's, is filled into the place of g - 1.  A wave waits for its own loads of stage g + 1
+// with those of the later ones under way, then for the other waves: one barrier a stage.  A load and a read of the next
+// step's fragment go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a SIMD
+// may have no other.  A tile's results go out through the ring's free place while the next tile's first stages come in.
 //
 // The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
 // counts its own, and waits that count more loads than it knows are longer, never shorter.
@@ -337,7 +347,7 @@ struct DirectLoader {
 
   // Lane by lane the pieces of LDS are filled in order; place() is its own inverse, so what belongs at place p of a row is
   // the row's piece place(p).
-  __device__ __forceinline__ DirectLoader(uint32_t rows, uint32_t stride) {
+  __device__ __forceinline__ void begin(uint32_t rows, uint32_t stride) {
 #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
       const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces;
@@ -355,7 +365,7 @@ struct DirectLoader {
   }
   // The last stage, of which only `depth` of k are there: by way of registers, with zeros behind.
   static __device__ __forceinline__ void load_partial(const T *__restrict__ base, uint32_t rows, size_t stride, uint32_t depth, T *lds) {
-#pragma unroll
+#pragma unroll 1
     for (uint32_t i = 0; i < kPieces; ++i) {
       const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces, piece = at % kRowPieces;
       typename Piece<T>::type v{};
@@ -369,50 +379,74 @@ struct DirectLoader {
   }
 };
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
-__device__ __forceinline__ void tile_product_direct(const T *__restrict__ a_, uint32_t rows, uint32_t a_stride,
-                                                    const T *__restrict__ b_, uint32_t cols, uint32_t b_stride, uint32_t depth,
-                                                    T *__restrict__ out, size_t out_stride, float4 *lds) {
+// A tile of a product: its operands' first elements, its extent and depth, and where its results go.
+template <typename T>
+struct Job {
+  const T *a, *b;
+  T *out;
+  uint32_t rows, cols, depth;
+};
+
+// job(n, &j): the workgroup's n-th tile; false: there are no more.
+template <typename T, bool A_ACROSS, bool B_ACROSS, typename S, typename JOBS>
+__device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_stride, uint32_t b_stride, size_t out_stride,
+                                                float4 *lds) {
   constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = kStageDepth / 2, kRing = S::kStages;
   constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
   static_assert((kRing & (kRing - 1)) == 0 && kRing >= 4, "a power of two");
-  const T *const a = uniform(a_), *const b = uniform(b_);
   T *const buffer = reinterpret_cast<T *>(lds);
   const uint32_t wave = uniform(threadIdx.x / kWave);
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
   const uint32_t lds_base = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float4 *)lds)));
-  Sums<T, S> sum = {};
   typedef DirectLoader<T, A_ACROSS, S::BM, S::kThreads> LoaderA;
   typedef DirectLoader<T, B_ACROSS, S::BN, S::kThreads> LoaderB;
-  const LoaderA load_a(rows, a_stride);
-  const LoaderB load_b(cols, b_stride);
   constexpr uint32_t kLoads = LoaderA::kPieces + LoaderB::kPieces;
-  const uint32_t whole = depth / kStageK<T>, stages = (depth + kStageK<T> - 1) / kStageK<T>;
   const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kStageK<T>;
   const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
 
-  const auto load_one = [&](uint32_t t, uint32_t i) {
-    const uint32_t to = lds_base + (t & (kRing - 1)) * kStageBytes;
-    if (i < LoaderA::kPieces)
-      load_a.load(i, a + t * a_step, to, wave);
-    else
-      load_b.load(i - LoaderA::kPieces, b + t * b_step, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
+  // what is filled: tile `filling`, from its stage `left` of `to_fill` on; `filled` and `done` count the stream's stages
+  Job<T> from;
+  LoaderA load_a;
+  LoaderB load_b;
+  uint32_t filling = 0, depth_left = 0, filled = 0, done = 0;
+  bool more = jobs(0, &from);
+  const auto begin = [&] {
+    load_a.begin(from.rows, a_stride);
+    load_b.begin(from.cols, b_stride);
+    depth_left = from.depth;
   };
-  const auto fill_rest = [&](uint32_t t) {  // a stage that may be partial, or none
-    T *const to = buffer + (t & (kRing - 1)) * (kA + kB);
-    if (t < whole) {
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) load_one(t, i);
-    } else if (t < stages) {
-      LoaderA::load_partial(a + t * a_step, rows, a_stride, depth - t * kStageK<T>, to);
-      LoaderB::load_partial(b + t * b_step, cols, b_stride, depth - t * kStageK<T>, to + kA);
+  if (more) begin();
+  const auto load_one = [&](uint32_t i) {
+    const uint32_t to = lds_base + (filled & (kRing - 1)) * kStageBytes;
+    if (i < LoaderA::kPieces)
+      load_a.load(i, from.a, to, wave);
+    else
+      load_b.load(i - LoaderA::kPieces, from.b, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
+  };
+  const auto filled_one = [&] {
+    from.a += a_step;
+    from.b += b_step;
+    depth_left -= kStageK<T> < depth_left ? kStageK<T> : depth_left;
+    ++filled;
+  };
+  const auto next_job = [&] {  // the next tile that has anything to fill
+    while (more && depth_left == 0) {
+      more = jobs(++filling, &from);
+      if (more) begin();
     }
   };
+  const auto fill_partial = [&] {
+    T *const to = buffer + (filled & (kRing - 1)) * (kA + kB);
+    LoaderA::load_partial(from.a, from.rows, a_stride, depth_left, to);
+    LoaderB::load_partial(from.b, from.cols, b_stride, depth_left, to + kA);
+    filled_one();
+  };
 
+  Sums<T, S> sum = {};
   typename Unit<T>::frag fa[2][S::kFragsM], fb[2][S::kFragsN];
   constexpr uint32_t kReads = S::kFragsM + S::kFragsN, kMuls = S::kFragsM * S::kFragsN;
-  const auto read_one = [&](uint32_t t, uint32_t step, uint32_t i) {
-    const T *const at = buffer + (t & (kRing - 1)) * (kA + kB);
+  const auto read_one = [&](uint32_t stage, uint32_t step, uint32_t i) {
+    const T *const at = buffer + (stage & (kRing - 1)) * (kA + kB);
     // (in the order in which the products need them)
     if (i == 0)
       fb[step & 1u][0] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0, step);
@@ -421,63 +455,111 @@ __device__ __forceinline__ void tile_product_direct(const T *__restrict__ a_, ui
     else
       fb[step & 1u][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0 + (i - S::kFragsM) * 32, step);
   };
-  // NEXT: there is a stage t + 1; FILL: and a whole one t + kRing - 1
-  const auto work = [&](uint32_t t, auto NEXT, auto FILL) {
+  // Stage `done`; FILL: there is a whole one to be filled.  `arrived`: stages up to this one are known to be there, whatever else is under way.
+  // Behind the stream's last stage something is read as well, which nothing uses.
+  uint32_t arrived = 0;
+  const auto work = [&](auto FILL) {
 #pragma unroll
     for (uint32_t step = 0; step < kSteps; ++step) {
       const bool last = step + 1 == kSteps;
-      if (last && NEXT.value) {  // stage t + 1 is there, and every wave holds its last fragments of stage t
-        wait_for_loads<FILL.value ? (kRing - 3) * kLoads + kLoads * (kSteps - 1) / kSteps : 0>();
+      if (last) {  // the next stage is there, and every wave holds its last fragments of this one
+        if (done + 1 >= arrived) {
+          wait_for_loads<FILL.value ? (kRing - 3) * kLoads + kLoads * (kSteps - 1) / kSteps : 0>();
+        }
         __syncthreads();
       }
 #pragma unroll
       for (uint32_t q = 0; q < kMuls; ++q) {
         const uint32_t i = q % S::kFragsM, j = q / S::kFragsM;
         sum[i][j] = Unit<T>::mul(fb[step & 1u][j], fa[step & 1u][i], sum[i][j]);
-        if (!last || NEXT.value) {
 #pragma unroll
-          for (uint32_t r = q * kReads / kMuls; r < (q + 1) * kReads / kMuls; ++r) read_one(last ? t + 1 : t, (step + 1) % kSteps, r);
-        }
-        if (FILL.value) {
-          constexpr uint32_t kShare = kLoads / kSteps;
-          static_assert(kLoads % kSteps == 0, "an equal share to a step");
+        for (uint32_t r = q * kReads / kMuls; r < (q + 1) * kReads / kMuls; ++r)
+          read_one(last ? done + 1 : done, (step + 1) % kSteps, r);
+        constexpr uint32_t kShare = kLoads / kSteps;
+        static_assert(kLoads % kSteps == 0, "an equal share to a step");
 #pragma unroll
-          for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r) load_one(t + kRing - 1, step * kShare + r);
-        }
+        for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r)
+          if (FILL.value) load_one(step * kShare + r);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if (FILL.value) filled_one();
+    ++done;
   };
 
+  for (uint32_t g = 0; g + 1 < kRing; ++g) {
+    next_job();
+    if (!more) break;
+    if (depth_left >= kStageK<T>) {
 #pragma unroll
-  for (uint32_t t = 0; t + 1 < kRing; ++t) fill_rest(t);
-  if (whole >= kRing - 1)
-    wait_for_loads<(kRing - 2) * kLoads>();
-  else
-    wait_for_loads<0>();
+      for (uint32_t i = 0; i < kLoads; ++i) load_one(i);
+      filled_one();
+    } else {
+      fill_partial();
+    }
+  }
+  wait_for_loads<0>();
   __syncthreads();
-  if (stages != 0) {
+  arrived = filled;
+  if (filled != 0) {
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
   }
-  uint32_t t = 0;
-  for (; t + kRing - 1 < whole; ++t) work(t, std::true_type(), std::true_type());
-  for (; t + 1 < stages; ++t) {
-    if (t + kRing - 1 == whole) fill_rest(t + kRing - 1);
-    work(t, std::true_type(), std::false_type());
+  Job<T> now;
+  for (uint32_t n = 0; jobs(n, &now); ++n) {
+    uint32_t left = (now.depth + kStageK<T> - 1) / kStageK<T>;
+    while (left != 0) {
+      next_job();
+      uint32_t turns = depth_left / kStageK<T>;  // stages with a whole one to fill
+      turns = turns < left ? turns : left;
+      left -= turns;
+      for (; turns != 0; --turns) work(std::true_type());
+      if (left != 0 && (!more || depth_left != 0)) {
+        if (more) fill_partial();
+        work(std::false_type());
+        --left;
+      }
+    }
+    wait_for_loads<0>();  // (stores are counted with the loads: from here on the stages up to `filled` are there)
+    arrived = filled;
+    constexpr uint32_t kRoom = kStageBytes / (S::WM * S::WN);
+    store_tile<T, S, kRoom>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
+                            buffer + ((done + kRing - 1) & (kRing - 1)) * (kA + kB) + wave * (kRoom / sizeof(T)));
+    __syncthreads();  // the free place is filled again
+#pragma unroll
+    for (uint32_t i = 0; i < S::kFragsM; ++i)
+#pragma unroll
+      for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = typename Unit<T>::acc{};
   }
-  if (t < stages) work(t, std::false_type(), std::false_type());
-  __syncthreads();
-  store_tile<T, S>(sum, rows, cols, out, out_stride, lds);
 }
 
-// Which tile a workgroup takes: those of a run lie on one XCD (workgroups go round the eight), where they share an L2.
-__device__ __forceinline__ uint32_t tile_of(uint32_t block, uint64_t tiles) {
-  const uint32_t share = static_cast<uint32_t>((tiles + 7) / 8);
-  const uint32_t index = block % 8 * share + block / 8;
-  return block / 8 < share && index < tiles ? index : kNoTile;
+// Tiles of a product: the run of XCD x of the eight (workgroups go round them) lies together, so that its tiles share an
+// L2; the XCD's workgroups take the run's tiles in turn.
+struct Turn {
+  uint32_t index, end, step;
+};
+__device__ __forceinline__ Turn turn_of(uint64_t tiles) {
+  const uint32_t share = static_cast<uint32_t>((tiles + 7) / 8), xcd = blockIdx.x % 8, n = static_cast<uint32_t>(tiles);
+  const uint32_t begin = xcd * share < n ? xcd * share : n;
+  return Turn{begin + blockIdx.x / 8, begin + share < n ? begin + share : n, gridDim.x / 8};
 }
-unsigned grid_of(uint64_t tiles) { return static_cast<unsigned>((tiles + 7) / 8 * 8); }
+
+// Rows from `first` on are zero: a workgroup takes a run of pieces of them.
+template <typename T>
+__device__ __forceinline__ void zero_from(T *__restrict__ out, uint32_t first, uint32_t rows, uint32_t cols, uint32_t threads) {
+  if (first >= rows) return;
+  const typename Piece<T>::type zero{};
+  T *const from = out + static_cast<size_t>(first) * cols;
+  const size_t n = static_cast<size_t>(rows - first) * cols;
+  const size_t step = static_cast<size_t>(gridDim.x) * threads * Piece<T>::kElems;
+  for (size_t at = (static_cast<size_t>(blockIdx.x) * threads + threadIdx.x) * Piece<T>::kElems; at < n; at += step) {
+    if (at + Piece<T>::kElems <= n) {
+      *reinterpret_cast<typename Piece<T>::type *>(from + at) = zero;
+    } else {
+      for (size_t j = at; j < n; ++j) from[j] = static_cast<T>(0.f);
+    }
+  }
+}
 
 template <typename T, bool OUT_MAJOR, typename S>
 __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
@@ -485,30 +567,35 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
                                                               uint32_t cols) {
   extern __shared__ float4 lds[];
+  __shared__ TileTable table;
   const uint32_t across = (cols + S::BN - 1) / S::BN;
-  uint32_t total;
-  TileFinder<S::kThreads> finder(indptr, experts, n_rows, S::BM, &total);
-  const uint32_t index = tile_of(blockIdx.x, static_cast<uint64_t>(total) * across);
-  if (index == kNoTile) return;
-  const Tile tile = finder.find(index / across);
-  const uint32_t col0 = uniform(index % across) * S::BN;
-  const uint32_t width = cols - col0 < S::BN ? cols - col0 : S::BN;
-  T *const to = out + static_cast<size_t>(tile.first) * cols + col0;
-  if (tile.expert >= experts) {  // rows behind the last expert's
-    typename Piece<T>::type zero{};
-    constexpr uint32_t kRow = S::BN / Piece<T>::kElems;
-    for (uint32_t at = threadIdx.x; at < (tile.end - tile.first) * kRow; at += S::kThreads)
-      if (at % kRow * Piece<T>::kElems < width)
-        store_piece<T>(to + static_cast<size_t>(at / kRow) * cols, at % kRow * Piece<T>::kElems, width, zero);
-    return;
+  const uint32_t total = table.build<S::kThreads>(indptr, experts, n_rows, S::BM);
+  const Turn turn = turn_of(static_cast<uint64_t>(total) * across);
+  const auto jobs = [&](uint32_t n, Job<T> *j) {
+    const uint32_t index = turn.index + n * turn.step;
+    if (index >= turn.end) return false;
+    const uint32_t down = uniform(index / across), col0 = (index - down * across) * S::BN;
+    const Tile tile = table.find(down, experts, S::BM);
+    const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
+    j->a = uniform(rows + static_cast<size_t>(tile.first) * inner);
+    j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
+    j->out = out + static_cast<size_t>(tile.first) * cols + col0;
+    j->rows = tile.end - tile.first;
+    j->cols = cols - col0 < S::BN ? cols - col0 : S::BN;
+    j->depth = inner;
+    return true;
+  };
+  if constexpr (S::kStages != 0) {
+    stream_products<T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds);
+  } else {
+    Job<T> j;
+    for (uint32_t n = 0; jobs(n, &j); ++n) {
+      tile_product<T, false, !OUT_MAJOR, S>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, inner, j.out, cols, lds);
+      __syncthreads();
+    }
   }
-  const T *const a = rows + static_cast<size_t>(tile.first) * inner;
-  const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
-  const T *const b = OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0;
-  if constexpr (S::kStages != 0)
-    tile_product_direct<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
-  else
-    tile_product<T, false, !OUT_MAJOR, S>(a, tile.end - tile.first, inner, b, width, OUT_MAJOR ? inner : cols, inner, to, cols, lds);
+  const uint32_t behind = indptr[experts];
+  zero_from(out, behind < n_rows ? behind : n_rows, n_rows, cols, S::kThreads);
 }
 
 // d_weight[expert] = left_e^T @ right_e over the expert's rows; (left, right) = (rows, ct), or (ct, rows) where the weight is
@@ -522,19 +609,30 @@ __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restri
   const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
   // An eighth of every expert's tiles to an XCD, neighbouring ones: the XCDs' work is the same however long the experts are.
   const uint32_t tiles = down * across, share = (tiles + 7) / 8;
-  const uint32_t expert = uniform(blockIdx.x / 8 / share);
-  const uint32_t in = (blockIdx.x + expert * tiles) % 8 * share + blockIdx.x / 8 % share;
-  if (in >= tiles) return;
-  const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
-  uint2 range = rows_of(indptr, expert, experts, n_rows);
-  range = make_uint2(uniform(range.x), uniform(range.y));
-  const T *const a = left + static_cast<size_t>(range.x) * n_left + p0, *const b = right + static_cast<size_t>(range.x) * n_right + q0;
-  const uint32_t high = n_left - p0 < S::BM ? n_left - p0 : S::BM, wide = n_right - q0 < S::BN ? n_right - q0 : S::BN;
-  T *const to = d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0;
-  if constexpr (S::kStages != 0)
-    tile_product_direct<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
-  else
-    tile_product<T, true, true, S>(a, high, n_left, b, wide, n_right, range.y - range.x, to, n_right, lds);
+  const auto jobs = [&](uint32_t n, Job<T> *j) {
+    const uint32_t expert = uniform(blockIdx.x / 8 / share);
+    const uint32_t in = (blockIdx.x + expert * tiles) % 8 * share + blockIdx.x / 8 % share;
+    if (n != 0 || in >= tiles) return false;
+    const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
+    uint2 range = rows_of(indptr, expert, experts, n_rows);
+    range = make_uint2(uniform(range.x), uniform(range.y));
+    j->a = uniform(left + static_cast<size_t>(range.x) * n_left + p0);
+    j->b = uniform(right + static_cast<size_t>(range.x) * n_right + q0);
+    j->out = d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0;
+    j->rows = n_left - p0 < S::BM ? n_left - p0 : S::BM;
+    j->cols = n_right - q0 < S::BN ? n_right - q0 : S::BN;
+    j->depth = range.y - range.x;
+    return true;
+  };
+  if constexpr (S::kStages != 0) {
+    stream_products<T, true, true, S>(jobs, n_left, n_right, n_right, lds);
+  } else {
+    Job<T> j;
+    for (uint32_t n = 0; jobs(n, &j); ++n) {
+      tile_product<T, true, true, S>(j.a, j.rows, n_left, j.b, j.cols, n_right, j.depth, j.out, n_right, lds);
+      __syncthreads();
+    }
+  }
 }
 
 bool refuse_grid(const char *target, uint64_t tiles) {
@@ -575,10 +673,16 @@ struct Staged {
 template <typename T, typename S>
 void launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
   const uint64_t tiles = most_tiles(d.rows, d.experts, S::BM) * div_up(d.out, S::BN);
-  if (refuse_grid(target, tiles)) return;
+  if (tiles >= 1ull << 32) {
+    set_error("%s: a product of %llu tiles is too large for one call", target, static_cast<unsigned long long>(tiles));
+    return;
+  }
+  // one workgroup to each place that the LDS leaves
+  const uint64_t places = static_cast<uint64_t>(device_info().num_cu) * (160u * 1024u / (S::kLdsBytes + sizeof(TileTable) + 1024u));
+  const unsigned grid = static_cast<unsigned>(((tiles < places ? tiles : places) + 7) / 8 * 8);
   const auto launch = [&](auto *kernel) {
     if (!allow_lds(target, kernel, S::kLdsBytes)) return;
-    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles)), dim3(S::kThreads), S::kLdsBytes, stream,
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLdsBytes, stream,
                        static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
                        static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
                        d.out);
