@@ -36,8 +36,7 @@ struct Tile {
   uint32_t expert, first, end;  // the rows of the tile: [first, end)
 };
 struct TileTable {
-  uint32_t start[kMostExperts + 1];
-  uint2 range[kMostExperts];
+  uint32_t start[kMostExperts];
   uint32_t wave_total[16];
 
   // the number of tiles
@@ -52,7 +51,6 @@ struct TileTable {
       own[j] = 0;
       if (j < per && e < experts) {
         const uint2 r = rows_of(indptr, e, experts, rows);
-        range[e] = r;
         own[j] = (r.y - r.x + height - 1) / height;
       }
       tiles += own[j];
@@ -78,14 +76,15 @@ struct TileTable {
 
   // index < the number of tiles; every wave by itself: the last expert that begins at or before it (those without tiles begin
   // where the next one does), 64 places and then 16 at a time
-  __device__ __forceinline__ Tile find(uint32_t index, uint32_t experts, uint32_t height) const {
+  __device__ __forceinline__ Tile find(const uint32_t *__restrict__ indptr, uint32_t index, uint32_t experts, uint32_t rows,
+                                       uint32_t height) const {
     static_assert(kMostExperts <= 64 * 16, "two looks are enough");
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t coarse = __popcll(__ballot(lane * 16 < experts && start[lane * 16 < experts ? lane * 16 : 0] <= index));
     const uint32_t e = (coarse - 1) * 16 + lane;
     const uint32_t fine = __popcll(__ballot(lane < 16 && e < experts && start[e < experts ? e : 0] <= index));
     const uint32_t expert = uniform((coarse - 1) * 16 + fine - 1);
-    const uint2 r = range[expert];
+    const uint2 r = rows_of(indptr, expert, experts, rows);
     const uint32_t first = uniform(r.x) + (index - uniform(start[expert])) * height, end = uniform(r.y);
     return Tile{expert, first, end - first < height ? end : first + height};
   }
@@ -208,7 +207,10 @@ __device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_
 template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t STAGES>
 struct Shape {
   static constexpr uint32_t kStages = STAGES;
-  static constexpr uint32_t kLdsBytes = (BM_ + BN_) * (STAGES != 0 ? STAGES * 64u : 2u * kDepthBytes);
+  // (a wave's room for its results: 32 rows of 64 columns in 16 bits; of 32 where two workgroups are to share a CU)
+  static constexpr uint32_t kRoom = BM_ * BN_ >= 256 * 256 ? 4096u : 2048u;
+  static constexpr uint32_t kRingBytes = (BM_ + BN_) * (STAGES != 0 ? STAGES : 2u) * kDepthBytes;
+  static constexpr uint32_t kLdsBytes = kRingBytes + (STAGES != 0 ? WM_ * WN_ * kRoom : 0u);
   static constexpr uint32_t BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * kWave;
   static constexpr uint32_t kFragsM = BM / WM / 32, kFragsN = BN / WN / 32;
 };
@@ -217,9 +219,10 @@ template <typename T, typename S>
 using Sums = typename Unit<T>::acc[S::kFragsM][S::kFragsN];
 
 // A wave's results to memory by way of a piece of LDS of its own, so that whole pieces of a row go side by side: a lane holds,
-// of row lane % 32, 4 neighbouring columns at a time.  kRoom bytes hold 32 rows of so many of the wave's columns.
+// of row lane % 32, 4 neighbouring columns at a time.  ROOM bytes hold 32 rows of so many of the wave's columns.  True: all of
+// the wave's results are there, and were stored in whole pieces.
 template <typename T, typename S, uint32_t ROOM>
-__device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols,
+__device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols,
                                            T *__restrict__ out, size_t out_stride, T *room) {
   constexpr uint32_t kElems = Piece<T>::kElems, kWide = S::BN / S::WN;
   constexpr uint32_t kCols = ROOM / 32 / sizeof(T) < kWide ? ROOM / 32 / sizeof(T) : kWide, kRow = kCols / kElems;
@@ -262,6 +265,7 @@ __device__ __forceinline__ void store_tile(const Sums<T, S> &sum, uint32_t m0, u
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  return whole;
 }
 
 // The tile's results to `out` (row-major, `stride` elements a row): `rows` x `cols` of it are there.
@@ -310,21 +314,22 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     }
     __syncthreads();
   }
-  constexpr uint32_t kRoom = S::kLdsBytes / (S::WM * S::WN) >= 8192 ? 8192 : S::kLdsBytes / (S::WM * S::WN);
-  store_tile<T, S, kRoom>(sum, m0, n0, rows, cols, out, out_stride, buffer + wave * (kRoom / sizeof(T)));
+  store_tile<T, S, S::kRoom>(sum, m0, n0, rows, cols, out, out_stride, buffer + wave * (S::kRoom / sizeof(T)));
 }
 
 // ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
 // For operands whose lines begin at multiples of 16 bytes.  A workgroup takes one tile after the other, and their stages
-// (64 bytes of a row of k each) are one stream through a ring of S::kStages places in LDS: stage g is worked on while stage
-// g + kStages - 1, perhaps the next tile's, is filled into the place of g - 1.  A wave waits for its own loads of stage g + 1
-// with those of the later ones under way, then for the other waves: one barrier a stage.  A load and a read of the next
-// step's fragment go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a SIMD
-// may have no other.  A tile's results go out through the ring's free place while the next tile's first stages come in.
+// (128 bytes of a row of k each, four steps of the matrix unit) are one stream through a ring of S::kStages places in LDS.
+//   step 0, 1   the fragments of the stage's other steps are read; then every wave holds all of the stage,
+//   step 2, 3   its place is filled with the stage that is kStages later, perhaps the next tile's,
+//   step 3      the next stage is waited for, with the later ones under way, and its first fragments are read.
+// Loads and reads go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a SIMD
+// may have no other.  (Stages of 64 bytes with four places leave the loads the same time, but ask the L2 twice as often.)
+// A tile's results go out by way of room of their own while the next tile's stages come in.
 //
 // The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
 // counts its own, and waits that count more loads than it knows are longer, never shorter.
-constexpr uint32_t kStageDepth = 4;  // pieces of 16 bytes
+constexpr uint32_t kStageDepth = 8;  // pieces of 16 bytes
 template <typename T>
 constexpr uint32_t kStageK = kStageDepth * Piece<T>::kElems;
 
@@ -393,7 +398,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
                                                 float4 *lds) {
   constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = kStageDepth / 2, kRing = S::kStages;
   constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
-  static_assert((kRing & (kRing - 1)) == 0 && kRing >= 4, "a power of two");
+  static_assert(kSteps == 4 && (kRing & (kRing - 1)) == 0 && kRing >= 2, "what work() goes by");
   T *const buffer = reinterpret_cast<T *>(lds);
   const uint32_t wave = uniform(threadIdx.x / kWave);
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
@@ -443,43 +448,55 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   };
 
   Sums<T, S> sum = {};
-  typename Unit<T>::frag fa[2][S::kFragsM], fb[2][S::kFragsN];
+  typename Unit<T>::frag fa[kSteps][S::kFragsM], fb[kSteps][S::kFragsN];
   constexpr uint32_t kReads = S::kFragsM + S::kFragsN, kMuls = S::kFragsM * S::kFragsN;
   const auto read_one = [&](uint32_t stage, uint32_t step, uint32_t i) {
     const T *const at = buffer + (stage & (kRing - 1)) * (kA + kB);
     // (in the order in which the products need them)
     if (i == 0)
-      fb[step & 1u][0] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0, step);
+      fb[step][0] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0, step);
     else if (i <= S::kFragsM)
-      fa[step & 1u][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth>(at, m0 + (i - 1) * 32, step);
+      fa[step][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth>(at, m0 + (i - 1) * 32, step);
     else
-      fb[step & 1u][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0 + (i - S::kFragsM) * 32, step);
+      fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0 + (i - S::kFragsM) * 32, step);
   };
-  // Stage `done`; FILL: there is a whole one to be filled.  `arrived`: stages up to this one are known to be there, whatever else is under way.
-  // Behind the stream's last stage something is read as well, which nothing uses.
-  uint32_t arrived = 0;
+  // Stage `done`, whose first fragments are held; FILL: there is a whole one to be filled.  `after`: stores that were issued
+  // after the loads of the next stage (the counter counts both, in the order in which they were issued).  Behind the stream's
+  // last stage something is read as well, which nothing uses.
+  constexpr uint32_t kStores = S::BM / S::WM * (S::BN / S::WN) / kWave / Piece<T>::kElems;  // of a wave's tile
+  bool after = false;
   const auto work = [&](auto FILL) {
 #pragma unroll
     for (uint32_t step = 0; step < kSteps; ++step) {
-      const bool last = step + 1 == kSteps;
-      if (last) {  // the next stage is there, and every wave holds its last fragments of this one
-        if (done + 1 >= arrived) {
-          wait_for_loads<FILL.value ? (kRing - 3) * kLoads + kLoads * (kSteps - 1) / kSteps : 0>();
-        }
+      if (step == 2) __syncthreads();  // every wave holds all of the stage
+      if (step == 2 && !FILL.value && more) fill_partial();
+      if (step == 3) {  // the next stage is there
+        constexpr uint32_t kUnderWay = FILL.value ? (kRing - 2) * kLoads + kLoads / 2 : 0;
+        if (FILL.value && after)
+          wait_for_loads<(kUnderWay + kStores < 63 ? kUnderWay + kStores : kUnderWay)>();
+        else
+          wait_for_loads<kUnderWay>();
+        after = false;
         __syncthreads();
       }
 #pragma unroll
       for (uint32_t q = 0; q < kMuls; ++q) {
         const uint32_t i = q % S::kFragsM, j = q / S::kFragsM;
-        sum[i][j] = Unit<T>::mul(fb[step & 1u][j], fa[step & 1u][i], sum[i][j]);
+        sum[i][j] = Unit<T>::mul(fb[step][j], fa[step][i], sum[i][j]);
+        const uint32_t reads = step == 0 ? 2 * kReads : step == 2 ? 0 : kReads;
 #pragma unroll
-        for (uint32_t r = q * kReads / kMuls; r < (q + 1) * kReads / kMuls; ++r)
-          read_one(last ? done + 1 : done, (step + 1) % kSteps, r);
-        constexpr uint32_t kShare = kLoads / kSteps;
-        static_assert(kLoads % kSteps == 0, "an equal share to a step");
+        for (uint32_t r = q * reads / kMuls; r < (q + 1) * reads / kMuls; ++r) {
+          if (step == 0)
+            read_one(done, 1 + r / kReads, r % kReads);
+          else
+            read_one(step == 1 ? done : done + 1, step == 1 ? 3 : 0, r);
+        }
+        constexpr uint32_t kShare = kLoads / 2;
+        static_assert(kLoads % 2 == 0, "an equal share to a step");
+        if (FILL.value && step >= 2) {
 #pragma unroll
-        for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r)
-          if (FILL.value) load_one(step * kShare + r);
+          for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r) load_one((step - 2) * kShare + r);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -487,7 +504,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
     ++done;
   };
 
-  for (uint32_t g = 0; g + 1 < kRing; ++g) {
+  for (uint32_t g = 0; g < kRing; ++g) {
     next_job();
     if (!more) break;
     if (depth_left >= kStageK<T>) {
@@ -500,11 +517,8 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   }
   wait_for_loads<0>();
   __syncthreads();
-  arrived = filled;
-  if (filled != 0) {
 #pragma unroll
-    for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
-  }
+  for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
   Job<T> now;
   for (uint32_t n = 0; jobs(n, &now); ++n) {
     uint32_t left = (now.depth + kStageK<T> - 1) / kStageK<T>;
@@ -515,17 +529,12 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
       left -= turns;
       for (; turns != 0; --turns) work(std::true_type());
       if (left != 0 && (!more || depth_left != 0)) {
-        if (more) fill_partial();
         work(std::false_type());
         --left;
       }
     }
-    wait_for_loads<0>();  // (stores are counted with the loads: from here on the stages up to `filled` are there)
-    arrived = filled;
-    constexpr uint32_t kRoom = kStageBytes / (S::WM * S::WN);
-    store_tile<T, S, kRoom>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
-                            buffer + ((done + kRing - 1) & (kRing - 1)) * (kA + kB) + wave * (kRoom / sizeof(T)));
-    __syncthreads();  // the free place is filled again
+    after = store_tile<T, S, S::kRoom>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
+                                       buffer + kRing * (kA + kB) + wave * (S::kRoom / sizeof(T)));
 #pragma unroll
     for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
@@ -575,7 +584,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
     const uint32_t index = turn.index + n * turn.step;
     if (index >= turn.end) return false;
     const uint32_t down = uniform(index / across), col0 = (index - down * across) * S::BN;
-    const Tile tile = table.find(down, experts, S::BM);
+    const Tile tile = table.find(indptr, down, experts, n_rows, S::BM);
     const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
     j->a = uniform(rows + static_cast<size_t>(tile.first) * inner);
     j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
@@ -660,9 +669,9 @@ bool whole_pieces(const void *p, uint32_t stride) {
 
 // Shapes for operands in whole pieces, and for others
 struct Direct {
-  using Large = Shape<256, 256, 2, 2, 4>;
-  using Middle = Shape<128, 128, 2, 2, 4>;
-  using Small = Shape<64, 64, 2, 2, 8>;
+  using Large = Shape<256, 256, 2, 2, 2>;
+  using Middle = Shape<128, 128, 2, 2, 2>;
+  using Small = Shape<64, 64, 2, 2, 4>;
 };
 struct Staged {
   using Large = Shape<256, 256, 2, 4, 0>;
