@@ -51,7 +51,7 @@ def lib():
                  "bpl_build_nonzero_descriptor", "bpl_build_jitconn_prob_homo_descriptor",
                  "bpl_build_jitconn_prob_uniform_descriptor", "bpl_build_jitconn_prob_normal_descriptor",
                  "bpl_build_matmat_jit_prob_descriptor1", "bpl_build_expert_descriptor",
-                 "bpl_expert_sort_scratch_bytes"):
+                 "bpl_expert_sort_scratch_bytes", "bpl_expert_matmul_gradient_scratch_bytes"):
       getattr(l, name).restype = ctypes.c_size_t
     _lib = l
   return _lib
@@ -237,3 +237,9 @@ def build_expert_descriptor(tokens, per_token, experts, rows, width, out_width, 
 @functools.lru_cache(maxsize=256)
 def expert_sort_scratch_bytes(pairs, experts):
   return lib().bpl_expert_sort_scratch_bytes(ctypes.c_uint32(pairs), ctypes.c_uint32(experts))
+
+
+@functools.lru_cache(maxsize=256)
+def expert_matmul_gradient_scratch_bytes(rows, experts, width, out_width, element_bytes):
+  u = ctypes.c_uint32
+  return lib().bpl_expert_matmul_gradient_scratch_bytes(u(rows), u(experts), u(width), u(out_width), u(element_bytes))

@@ -103,31 +103,32 @@ uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
 //   across: LDS holds [k][m]; 16-bit types are transposed by the LDS's transposing read (16 lanes read 4 rows of 16
 //           elements and get a column of 4 each), 32-bit ones are read one by one.
 // 16-byte pieces are placed so that the lanes of a read meet different banks (place()).
-template <typename T>
-struct Unit;  // the matrix instructions of a type: one piece of k (kPieceK elements) of 32 x 32 results
-template <>
-struct Unit<half_t> {
-  typedef half_t frag __attribute__((ext_vector_type(8)));
-  typedef float acc __attribute__((ext_vector_type(16)));
-  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-};
-template <>
-struct Unit<bfloat_t> {
-  typedef bfloat_t frag __attribute__((ext_vector_type(8)));
-  typedef float acc __attribute__((ext_vector_type(16)));
-  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-};
-template <>
-struct Unit<float> {
-  typedef float frag __attribute__((ext_vector_type(4)));
-  typedef float acc __attribute__((ext_vector_type(16)));
-  // (four steps of k = 2: the lower lanes hold k 0 to 3 of the piece, the upper 4 to 7; both operands alike)
-  static __device__ __forceinline__ acc mul(frag a, frag b, acc c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-};
+template <typename T, uint32_t SIDE>
+struct Unit;  // the matrix instructions of a type: SIDE x SIDE results, one piece (16 bytes) of k from each of the 64 / SIDE lanes of a row
+#define BPL_UNIT16(TYPE, SIDE, LENGTH, INSTRUCTION)                                                                        \
+  template <>                                                                                                              \
+  struct Unit<TYPE, SIDE> {                                                                                                \
+    typedef TYPE frag __attribute__((ext_vector_type(8)));                                                                 \
+    typedef float acc __attribute__((ext_vector_type(LENGTH)));                                                            \
+    static __device__ __forceinline__ acc mul(frag a, frag b, acc c) { return INSTRUCTION(a, b, c, 0, 0, 0); }             \
+  };
+BPL_UNIT16(half_t, 32, 16, __builtin_amdgcn_mfma_f32_32x32x16_f16)
+BPL_UNIT16(half_t, 16, 4, __builtin_amdgcn_mfma_f32_16x16x32_f16)
+BPL_UNIT16(bfloat_t, 32, 16, __builtin_amdgcn_mfma_f32_32x32x16_bf16)
+BPL_UNIT16(bfloat_t, 16, 4, __builtin_amdgcn_mfma_f32_16x16x32_bf16)
+// (in 32 bits four instructions of one k a lane each; which k a lane holds is the same for both operands, and no matter else)
+#define BPL_UNIT32(SIDE, LENGTH, INSTRUCTION)                                    \
+  template <>                                                                    \
+  struct Unit<float, SIDE> {                                                     \
+    typedef float frag __attribute__((ext_vector_type(4)));                      \
+    typedef float acc __attribute__((ext_vector_type(LENGTH)));                  \
+    static __device__ __forceinline__ acc mul(frag a, frag b, acc c) {           \
+      _Pragma("unroll") for (int j = 0; j < 4; ++j) c = INSTRUCTION(a[j], b[j], c, 0, 0, 0); \
+      return c;                                                                  \
+    }                                                                            \
+  };
+BPL_UNIT32(32, 16, __builtin_amdgcn_mfma_f32_32x32x2f32)
+BPL_UNIT32(16, 4, __builtin_amdgcn_mfma_f32_16x16x4f32)
 
 constexpr uint32_t kDepthBytes = 128;
 template <typename T>
@@ -177,24 +178,24 @@ struct Loader {
   }
 };
 
-// What a lane gives the matrix unit: of row `row0` + lane % 32, piece 2 * step + lane / 32 of k.
-template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH>
-__device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_t row0, uint32_t step) {
-  typedef typename Unit<T>::frag frag;
-  const uint32_t lane = threadIdx.x % kWave;
+// What a lane gives the matrix unit: of row `row0` + lane % SIDE, piece (64 / SIDE) * step + lane / SIDE of k.
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH, uint32_t SIDE>
+__device__ __forceinline__ typename Unit<T, SIDE>::frag fragment(const T *lds, uint32_t row0, uint32_t step) {
+  typedef typename Unit<T, SIDE>::frag frag;
+  const uint32_t lane = threadIdx.x % kWave, piece = kWave / SIDE * step + lane / SIDE;
   if constexpr (!ACROSS) {
-    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH, DEPTH>(row0 + lane % 32, 2 * step + lane / 32)]);
+    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH, DEPTH>(row0 + lane % SIDE, piece)]);
   } else if constexpr (sizeof(T) == 4) {
     frag f;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) f[j] = lds[(step * 8 + lane / 32 * 4 + j) * WIDTH + row0 + lane % 32];
+    for (uint32_t j = 0; j < 4; ++j) f[j] = lds[(piece * 4 + j) * WIDTH + row0 + lane % SIDE];
     return f;
   } else {
     typedef short quad __attribute__((ext_vector_type(4)));
     quad half[2];
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) {
-      const uint32_t k = step * 16 + lane / 32 * 8 + j * 4 + lane % 16 / 4, col = row0 + lane % 32 / 16 * 16 + lane % 4 * 4;
+      const uint32_t k = piece * 8 + j * 4 + lane % 16 / 4, col = row0 + lane % SIDE / 16 * 16 + lane % 4 * 4;
       const T *from = lds + place<T, true, WIDTH, DEPTH>(k, col / 8) * 8 + col % 8;
       half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) quad *)from);
     }
@@ -202,32 +203,33 @@ __device__ __forceinline__ typename Unit<T>::frag fragment(const T *lds, uint32_
   }
 }
 
-// Shape of a tile: BM x BN results, WM x WN waves; kStages: of the ring of loads that go straight to LDS, 0: staged through
+// Shape of a tile: BM x BN results, WM x WN waves, matrix instructions of SIDE x SIDE; kStages: of the ring of loads that go straight to LDS, 0: staged through
 // registers into two buffers.
-template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t STAGES>
+template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t SIDE, uint32_t STAGES>
 struct Shape {
+  static constexpr uint32_t kSide = SIDE, kSteps = kDepthBytes / 16 / (kWave / SIDE);
   static constexpr uint32_t kStages = STAGES;
-  // (a wave's room for its results: 32 rows of 64 columns in 16 bits; of 32 where two workgroups are to share a CU)
-  static constexpr uint32_t kRoom = BM_ * BN_ >= 256 * 256 ? 4096u : 2048u;
+  // (a wave's room for its results: SIDE rows of 64 columns in 16 bits; of 32 where workgroups are to share a CU)
+  static constexpr uint32_t kRoom = BM_ * BN_ >= 256 * 256 ? 4096u : SIDE * 64u;
   static constexpr uint32_t kRingBytes = (BM_ + BN_) * (STAGES != 0 ? STAGES : 2u) * kDepthBytes;
   static constexpr uint32_t kLdsBytes = kRingBytes + (STAGES != 0 ? WM_ * WN_ * kRoom : 0u);
   static constexpr uint32_t BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * kWave;
-  static constexpr uint32_t kFragsM = BM / WM / 32, kFragsN = BN / WN / 32;
+  static constexpr uint32_t kFragsM = BM / WM / SIDE, kFragsN = BN / WN / SIDE;
 };
 
 template <typename T, typename S>
-using Sums = typename Unit<T>::acc[S::kFragsM][S::kFragsN];
+using Sums = typename Unit<T, S::kSide>::acc[S::kFragsM][S::kFragsN];
 
 // A wave's results to memory by way of a piece of LDS of its own, so that whole pieces of a row go side by side: a lane holds,
-// of row lane % 32, 4 neighbouring columns at a time.  ROOM bytes hold 32 rows of so many of the wave's columns.  True: all of
+// of row lane % kSide, 4 neighbouring columns at a time.  ROOM bytes hold kSide rows of so many of the wave's columns.  True: all of
 // the wave's results are there, and were stored in whole pieces.
-template <typename T, typename S, uint32_t ROOM>
+template <typename T, typename S, uint32_t ROOM, typename O>
 __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols,
-                                           T *__restrict__ out, size_t out_stride, T *room) {
-  constexpr uint32_t kElems = Piece<T>::kElems, kWide = S::BN / S::WN;
-  constexpr uint32_t kCols = ROOM / 32 / sizeof(T) < kWide ? ROOM / 32 / sizeof(T) : kWide, kRow = kCols / kElems;
-  static_assert(kCols % 8 == 0 && kWide % kCols == 0 && (kRow & (kRow - 1)) == 0, "whole groups of 8 columns");
-  typedef T quad __attribute__((ext_vector_type(4)));
+                                           O *__restrict__ out, size_t out_stride, O *room) {
+  constexpr uint32_t kElems = Piece<O>::kElems, kWide = S::BN / S::WN, kSide = S::kSide, kGroup = kWave / kSide * 4;
+  constexpr uint32_t kCols = ROOM / kSide / sizeof(O) < kWide ? ROOM / kSide / sizeof(O) : kWide, kRow = kCols / kElems;
+  static_assert(kCols % kGroup == 0 && kWide % kCols == 0 && (kRow & (kRow - 1)) == 0 && kWave % kRow == 0, "whole groups of columns");
+  typedef O quad __attribute__((ext_vector_type(4)));
   const uint32_t lane = threadIdx.x % kWave;
   const bool whole = m0 + S::BM / S::WM <= rows && n0 + kWide <= cols;
 #pragma unroll
@@ -235,12 +237,12 @@ __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, u
 #pragma unroll
     for (uint32_t c0 = 0; c0 < kWide; c0 += kCols) {
 #pragma unroll
-      for (uint32_t g = 0; g < kCols / 8; ++g) {
-        const uint32_t j = (c0 / 8 + g) / 4, r = (c0 / 8 + g) % 4;
+      for (uint32_t g = 0; g < kCols / kGroup; ++g) {
+        const uint32_t j = (c0 / kGroup + g) * kGroup / kSide, r = (c0 / kGroup + g) % (kSide / kGroup);
         quad v;
 #pragma unroll
-        for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<T>(sum[i][j][r * 4 + c]);
-        const uint32_t row = lane % 32, col = g * 8 + lane / 32 * 4;
+        for (uint32_t c = 0; c < 4; ++c) v[c] = static_cast<O>(sum[i][j][r * 4 + c]);
+        const uint32_t row = lane % kSide, col = g * kGroup + lane / kSide * 4;
         // (pieces are placed by the row, against bank conflicts)
         *reinterpret_cast<quad *>(room + (row * kRow + ((col / kElems) ^ (row & (kRow - 1)))) * kElems + col % kElems) = v;
       }
@@ -250,16 +252,16 @@ __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, u
       constexpr uint32_t kRows = kWave / kRow;  // that the lanes hold at a time
       const uint32_t row0 = lane / kRow, piece = lane % kRow, n = n0 + c0 + piece * kElems;
       const auto held = [&](uint32_t row) {
-        return __builtin_bit_cast(typename Piece<T>::type, reinterpret_cast<const float4 *>(room)[row * kRow + (piece ^ (row & (kRow - 1)))]);
+        return __builtin_bit_cast(typename Piece<O>::type, reinterpret_cast<const float4 *>(room)[row * kRow + (piece ^ (row & (kRow - 1)))]);
       };
-      T *const to = out + (m0 + i * 32 + row0) * out_stride + n;
+      O *const to = out + (m0 + i * kSide + row0) * out_stride + n;
       if (whole) {
 #pragma unroll
-        for (uint32_t p = 0; p < 32; p += kRows) *reinterpret_cast<typename Piece<T>::type *>(to + p * out_stride) = held(p + row0);
+        for (uint32_t p = 0; p < kSide; p += kRows) *reinterpret_cast<typename Piece<O>::type *>(to + p * out_stride) = held(p + row0);
       } else {
 #pragma unroll 1
-        for (uint32_t p = 0; p < 32; p += kRows)
-          if (m0 + i * 32 + p + row0 < rows && n < cols) store_piece<T>(to + p * out_stride - n, n, cols, held(p + row0));
+        for (uint32_t p = 0; p < kSide; p += kRows)
+          if (m0 + i * kSide + p + row0 < rows && n < cols) store_piece<O>(to + p * out_stride - n, n, cols, held(p + row0));
       }
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_sched_barrier(0);
@@ -269,15 +271,15 @@ __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, u
 }
 
 // The tile's results to `out` (row-major, `stride` elements a row): `rows` x `cols` of it are there.
-template <typename T, bool A_ACROSS, bool B_ACROSS, typename S>
+template <typename T, bool A_ACROSS, bool B_ACROSS, typename S, typename O>
 __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t rows, size_t a_stride, const T *__restrict__ b,
-                                             uint32_t cols, size_t b_stride, uint32_t depth, T *__restrict__ out,
+                                             uint32_t cols, size_t b_stride, uint32_t depth, O *__restrict__ out,
                                              size_t out_stride, float4 *lds) {
-  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = 4;
+  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = S::kSteps, kSide = S::kSide;
   T *const buffer = reinterpret_cast<T *>(lds);  // A, B of one buffer, then of the other
   const uint32_t wave = threadIdx.x / kWave;
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
-  typename Unit<T>::acc sum[S::kFragsM][S::kFragsN] = {};
+  typename Unit<T, S::kSide>::acc sum[S::kFragsM][S::kFragsN] = {};
   Loader<T, A_ACROSS, S::BM, S::kThreads> load_a;
   Loader<T, B_ACROSS, S::BN, S::kThreads> load_b;
   if (depth != 0) {
@@ -297,15 +299,15 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     const T *const at = buffer + turn * (kA + kB);
 #pragma unroll
     for (uint32_t step = 0; step < kSteps; ++step) {
-      typename Unit<T>::frag fa[S::kFragsM], fb[S::kFragsN];
+      typename Unit<T, S::kSide>::frag fa[S::kFragsM], fb[S::kFragsN];
 #pragma unroll
-      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM, 8>(at, m0 + i * 32, step);
+      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM, 8, kSide>(at, m0 + i * kSide, step);
 #pragma unroll
-      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN, 8>(at + kA, n0 + j * 32, step);
+      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN, 8, kSide>(at + kA, n0 + j * kSide, step);
 #pragma unroll
       for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
-        for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = Unit<T>::mul(fb[j], fa[i], sum[i][j]);
+        for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = Unit<T, S::kSide>::mul(fb[j], fa[i], sum[i][j]);
     }
     if (more) {
       T *const to = buffer + (turn ^ 1u) * (kA + kB);
@@ -314,7 +316,8 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     }
     __syncthreads();
   }
-  store_tile<T, S, S::kRoom>(sum, m0, n0, rows, cols, out, out_stride, buffer + wave * (S::kRoom / sizeof(T)));
+  store_tile<T, S, S::kRoom, O>(sum, m0, n0, rows, cols, out, out_stride,
+                             reinterpret_cast<O *>(buffer) + wave * (S::kRoom / sizeof(O)));
 }
 
 // ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
@@ -323,6 +326,7 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
 //   step 0, 1   the fragments of the stage's other steps are read; then every wave holds all of the stage,
 //   step 2, 3   its place is filled with the stage that is kStages later, perhaps the next tile's,
 //   step 3      the next stage is waited for, with the later ones under way, and its first fragments are read.
+// (Instructions of 16 x 16 take the stage in two steps, each twice as deep.)
 // Loads and reads go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a SIMD
 // may have no other.  (Stages of 64 bytes with four places leave the loads the same time, but ask the L2 twice as often.)
 // A tile's results go out by way of room of their own while the next tile's stages come in.
@@ -385,20 +389,20 @@ struct DirectLoader {
 };
 
 // A tile of a product: its operands' first elements, its extent and depth, and where its results go.
-template <typename T>
+template <typename T, typename O>
 struct Job {
   const T *a, *b;
-  T *out;
+  O *out;
   uint32_t rows, cols, depth;
 };
 
 // job(n, &j): the workgroup's n-th tile; false: there are no more.
-template <typename T, bool A_ACROSS, bool B_ACROSS, typename S, typename JOBS>
+template <typename T, typename O, bool A_ACROSS, bool B_ACROSS, typename S, typename JOBS>
 __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_stride, uint32_t b_stride, size_t out_stride,
                                                 float4 *lds) {
-  constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = kStageDepth / 2, kRing = S::kStages;
+  constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = S::kSteps, kSide = S::kSide, kRing = S::kStages;
   constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
-  static_assert(kSteps == 4 && (kRing & (kRing - 1)) == 0 && kRing >= 2, "what work() goes by");
+  static_assert((kSteps == 4 || kSteps == 2) && (kRing & (kRing - 1)) == 0 && kRing >= 2, "what work() goes by");
   T *const buffer = reinterpret_cast<T *>(lds);
   const uint32_t wave = uniform(threadIdx.x / kWave);
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
@@ -410,7 +414,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
 
   // what is filled: tile `filling`, from its stage `left` of `to_fill` on; `filled` and `done` count the stream's stages
-  Job<T> from;
+  Job<T, O> from;
   LoaderA load_a;
   LoaderB load_b;
   uint32_t filling = 0, depth_left = 0, filled = 0, done = 0;
@@ -448,30 +452,32 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   };
 
   Sums<T, S> sum = {};
-  typename Unit<T>::frag fa[kSteps][S::kFragsM], fb[kSteps][S::kFragsN];
+  typename Unit<T, S::kSide>::frag fa[kSteps][S::kFragsM], fb[kSteps][S::kFragsN];
   constexpr uint32_t kReads = S::kFragsM + S::kFragsN, kMuls = S::kFragsM * S::kFragsN;
   const auto read_one = [&](uint32_t stage, uint32_t step, uint32_t i) {
     const T *const at = buffer + (stage & (kRing - 1)) * (kA + kB);
     // (in the order in which the products need them)
     if (i == 0)
-      fb[step][0] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0, step);
+      fb[step][0] = fragment<T, B_ACROSS, S::BN, kStageDepth, kSide>(at + kA, n0, step);
     else if (i <= S::kFragsM)
-      fa[step][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth>(at, m0 + (i - 1) * 32, step);
+      fa[step][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth, kSide>(at, m0 + (i - 1) * kSide, step);
     else
-      fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth>(at + kA, n0 + (i - S::kFragsM) * 32, step);
+      fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth, kSide>(at + kA, n0 + (i - S::kFragsM) * kSide, step);
   };
   // Stage `done`, whose first fragments are held; FILL: there is a whole one to be filled.  `after`: stores that were issued
   // after the loads of the next stage (the counter counts both, in the order in which they were issued).  Behind the stream's
   // last stage something is read as well, which nothing uses.
-  constexpr uint32_t kStores = S::BM / S::WM * (S::BN / S::WN) / kWave / Piece<T>::kElems;  // of a wave's tile
+  constexpr uint32_t kStores = S::BM / S::WM * (S::BN / S::WN) / kWave / Piece<O>::kElems;  // of a wave's tile
   bool after = false;
   const auto work = [&](auto FILL) {
 #pragma unroll
     for (uint32_t step = 0; step < kSteps; ++step) {
-      if (step == 2) __syncthreads();  // every wave holds all of the stage
-      if (step == 2 && !FILL.value && more) fill_partial();
-      if (step == 3) {  // the next stage is there
-        constexpr uint32_t kUnderWay = FILL.value ? (kRing - 2) * kLoads + kLoads / 2 : 0;
+      const bool last = step + 1 == kSteps;
+      if (step == kSteps / 2) {
+        if (!last) __syncthreads();  // every wave holds all of the stage
+      }
+      if (last) {  // the next stage is there (and, of two steps, every wave holds all of this one)
+        constexpr uint32_t kUnderWay = FILL.value ? (kRing - 2) * kLoads + (kSteps == 4 ? kLoads / 2 : 0) : 0;
         if (FILL.value && after)
           wait_for_loads<(kUnderWay + kStores < 63 ? kUnderWay + kStores : kUnderWay)>();
         else
@@ -479,23 +485,27 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
         after = false;
         __syncthreads();
       }
+      if (step == kSteps / 2 && !FILL.value && more) fill_partial();
 #pragma unroll
       for (uint32_t q = 0; q < kMuls; ++q) {
         const uint32_t i = q % S::kFragsM, j = q / S::kFragsM;
-        sum[i][j] = Unit<T>::mul(fb[step][j], fa[step][i], sum[i][j]);
-        const uint32_t reads = step == 0 ? 2 * kReads : step == 2 ? 0 : kReads;
+        sum[i][j] = Unit<T, S::kSide>::mul(fb[step][j], fa[step][i], sum[i][j]);
+        // of four steps: 1 and 2 are read in 0, 3 in 1, the next stage's 0 in 3; of two: 1 in 0, the next stage's 0 in 1
+        const uint32_t reads = kSteps == 4 ? (step == 0 ? 2 * kReads : step == 2 ? 0 : kReads) : kReads;
 #pragma unroll
         for (uint32_t r = q * reads / kMuls; r < (q + 1) * reads / kMuls; ++r) {
-          if (step == 0)
+          if (last)
+            read_one(done + 1, 0, r);
+          else if (step == 0)
             read_one(done, 1 + r / kReads, r % kReads);
           else
-            read_one(step == 1 ? done : done + 1, step == 1 ? 3 : 0, r);
+            read_one(done, 3, r);
         }
-        constexpr uint32_t kShare = kLoads / 2;
-        static_assert(kLoads % 2 == 0, "an equal share to a step");
-        if (FILL.value && step >= 2) {
+        if (FILL.value && step >= kSteps / 2) {
+          constexpr uint32_t kShare = kLoads / (kSteps / 2);
+          static_assert(kLoads % (kSteps / 2) == 0, "an equal share to a step");
 #pragma unroll
-          for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r) load_one((step - 2) * kShare + r);
+          for (uint32_t r = q * kShare / kMuls; r < (q + 1) * kShare / kMuls; ++r) load_one((step - kSteps / 2) * kShare + r);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -519,7 +529,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
-  Job<T> now;
+  Job<T, O> now;
   for (uint32_t n = 0; jobs(n, &now); ++n) {
     uint32_t left = (now.depth + kStageK<T> - 1) / kStageK<T>;
     while (left != 0) {
@@ -533,12 +543,12 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
         --left;
       }
     }
-    after = store_tile<T, S, S::kRoom>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
-                                       buffer + kRing * (kA + kB) + wave * (S::kRoom / sizeof(T)));
+    after = store_tile<T, S, S::kRoom, O>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
+                                       reinterpret_cast<O *>(buffer + kRing * (kA + kB)) + wave * (S::kRoom / sizeof(O)));
 #pragma unroll
     for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
-      for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = typename Unit<T>::acc{};
+      for (uint32_t j = 0; j < S::kFragsN; ++j) sum[i][j] = typename Unit<T, S::kSide>::acc{};
   }
 }
 
@@ -580,7 +590,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
   const uint32_t across = (cols + S::BN - 1) / S::BN;
   const uint32_t total = table.build<S::kThreads>(indptr, experts, n_rows, S::BM);
   const Turn turn = turn_of(static_cast<uint64_t>(total) * across);
-  const auto jobs = [&](uint32_t n, Job<T> *j) {
+  const auto jobs = [&](uint32_t n, Job<T, T> *j) {
     const uint32_t index = turn.index + n * turn.step;
     if (index >= turn.end) return false;
     const uint32_t down = uniform(index / across), col0 = (index - down * across) * S::BN;
@@ -595,11 +605,11 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
     return true;
   };
   if constexpr (S::kStages != 0) {
-    stream_products<T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds);
+    stream_products<T, T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds);
   } else {
-    Job<T> j;
+    Job<T, T> j;
     for (uint32_t n = 0; jobs(n, &j); ++n) {
-      tile_product<T, false, !OUT_MAJOR, S>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, inner, j.out, cols, lds);
+      tile_product<T, false, !OUT_MAJOR, S, T>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, inner, j.out, cols, lds);
       __syncthreads();
     }
   }
@@ -608,44 +618,61 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
 }
 
 // d_weight[expert] = left_e^T @ right_e over the expert's rows; (left, right) = (rows, ct), or (ct, rows) where the weight is
-// stored out-major.
-template <typename T, typename S>
+// stored out-major.  Where there are few tiles an expert's rows are split into `parts`: O = float, part after part, and
+// join_kernel adds them in their order.
+template <typename T, typename O, typename S>
 __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
-                                                               const uint32_t *__restrict__ indptr, T *__restrict__ d_weight,
+                                                               const uint32_t *__restrict__ indptr, O *__restrict__ d_weight,
                                                                uint32_t n_rows, uint32_t experts, uint32_t n_left,
-                                                               uint32_t n_right) {
+                                                               uint32_t n_right, uint32_t parts) {
   extern __shared__ float4 lds[];
   const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
   // An eighth of every expert's tiles to an XCD, neighbouring ones: the XCDs' work is the same however long the experts are.
   const uint32_t tiles = down * across, share = (tiles + 7) / 8;
-  const auto jobs = [&](uint32_t n, Job<T> *j) {
-    const uint32_t expert = uniform(blockIdx.x / 8 / share);
-    const uint32_t in = (blockIdx.x + expert * tiles) % 8 * share + blockIdx.x / 8 % share;
+  const auto jobs = [&](uint32_t n, Job<T, O> *j) {
+    const uint32_t which = uniform(blockIdx.x / 8 / share), expert = uniform(which / parts), part = which - expert * parts;
+    const uint32_t in = (blockIdx.x + which * tiles) % 8 * share + blockIdx.x / 8 % share;
     if (n != 0 || in >= tiles) return false;
     const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
     uint2 range = rows_of(indptr, expert, experts, n_rows);
+    if (parts != 1) {  // whole stages to a part
+      const uint32_t length = ((range.y - range.x + parts - 1) / parts + kDepth<T> - 1) / kDepth<T> * kDepth<T>;
+      const uint64_t from = static_cast<uint64_t>(range.x) + static_cast<uint64_t>(length) * part;
+      range.x = from < range.y ? static_cast<uint32_t>(from) : range.y;
+      range.y = range.y - range.x < length ? range.y : range.x + length;
+    }
     range = make_uint2(uniform(range.x), uniform(range.y));
     j->a = uniform(left + static_cast<size_t>(range.x) * n_left + p0);
     j->b = uniform(right + static_cast<size_t>(range.x) * n_right + q0);
-    j->out = d_weight + (static_cast<size_t>(expert) * n_left + p0) * n_right + q0;
+    j->out = d_weight + ((static_cast<size_t>(part) * experts + expert) * n_left + p0) * n_right + q0;
     j->rows = n_left - p0 < S::BM ? n_left - p0 : S::BM;
     j->cols = n_right - q0 < S::BN ? n_right - q0 : S::BN;
     j->depth = range.y - range.x;
     return true;
   };
   if constexpr (S::kStages != 0) {
-    stream_products<T, true, true, S>(jobs, n_left, n_right, n_right, lds);
+    stream_products<T, O, true, true, S>(jobs, n_left, n_right, n_right, lds);
   } else {
-    Job<T> j;
+    Job<T, O> j;
     for (uint32_t n = 0; jobs(n, &j); ++n) {
-      tile_product<T, true, true, S>(j.a, j.rows, n_left, j.b, j.cols, n_right, j.depth, j.out, n_right, lds);
+      tile_product<T, true, true, S, O>(j.a, j.rows, n_left, j.b, j.cols, n_right, j.depth, j.out, n_right, lds);
       __syncthreads();
     }
   }
 }
 
-bool refuse_grid(const char *target, uint64_t tiles) {
-  if (tiles < (1u << 22)) return false;  // (threads of a launch are counted in 32 bits)
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ parts, T *__restrict__ out, size_t n, uint32_t count) {
+  for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * 256) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (uint32_t p = 0; p < count; ++p) sum += parts[p * n + i];
+    out[i] = static_cast<T>(sum);
+  }
+}
+
+bool refuse_tiles(const char *target, uint64_t tiles, uint64_t most) {
+  if (tiles < most) return false;
   set_error("%s: a product of %llu tiles is too large for one call", target, static_cast<unsigned long long>(tiles));
   return true;
 }
@@ -669,23 +696,22 @@ bool whole_pieces(const void *p, uint32_t stride) {
 
 // Shapes for operands in whole pieces, and for others
 struct Direct {
-  using Large = Shape<256, 256, 2, 2, 2>;
-  using Middle = Shape<128, 128, 2, 2, 2>;
-  using Small = Shape<64, 64, 2, 2, 4>;
+  using Large = Shape<256, 256, 2, 2, 32, 2>;
+  using Middle = Shape<128, 128, 2, 2, 32, 2>;
+  using Small = Shape<64, 64, 2, 2, 32, 4>;
+  using Thin = Shape<16, 64, 1, 2, 16, 4>;
 };
 struct Staged {
-  using Large = Shape<256, 256, 2, 4, 0>;
-  using Middle = Shape<128, 128, 2, 2, 0>;
-  using Small = Shape<64, 64, 2, 2, 0>;
+  using Large = Shape<256, 256, 2, 4, 32, 0>;
+  using Middle = Shape<128, 128, 2, 2, 32, 0>;
+  using Small = Shape<64, 64, 2, 2, 32, 0>;
+  using Thin = Shape<16, 64, 1, 2, 16, 0>;
 };
 
 template <typename T, typename S>
 void launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
   const uint64_t tiles = most_tiles(d.rows, d.experts, S::BM) * div_up(d.out, S::BN);
-  if (tiles >= 1ull << 32) {
-    set_error("%s: a product of %llu tiles is too large for one call", target, static_cast<unsigned long long>(tiles));
-    return;
-  }
+  if (refuse_tiles(target, tiles, 1ull << 32)) return;
   // one workgroup to each place that the LDS leaves
   const uint64_t places = static_cast<uint64_t>(device_info().num_cu) * (160u * 1024u / (S::kLdsBytes + sizeof(TileTable) + 1024u));
   const unsigned grid = static_cast<unsigned>(((tiles < places ? tiles : places) + 7) / 8 * 8);
@@ -703,13 +729,47 @@ void launch_product(const char *target, hipStream_t stream, const bpl_expert_des
     launch(product_kernel<T, false, S>);
 }
 
+// Which shape: the least time by the tiles that a CU works through one after the other (those that share it, at least) and a
+// tile's time, measured with the card full of them (32,768 rows, 64 experts, inner dimension 2,048, bfloat16: 60, 19 and 8.5 us;
+// in 32 bits, inner dimension 1,024: 61, 17 and 6 us for the middle, the small and the thin one).  Mean rows of an expert
+// and times of the shapes at 1,536 columns, bfloat16, large / middle / small: 512 rows 239 / 260 / 432, 128 rows 131 / 118 /
+// 147, 16 rows 119 / 86 / 78 us; float32, 1,024 columns, middle / small / thin: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
+enum Form { kLarge, kMiddle, kSmall, kThin };
+struct FormTime {
+  Form form;
+  uint32_t height, width, share;  // share: workgroups that share a CU
+  float time;
+};
+constexpr FormTime kForms16[] = {{kLarge, 256, 256, 1, 60.f}, {kMiddle, 128, 128, 2, 19.f}, {kSmall, 64, 64, 2, 8.5f}};
+constexpr FormTime kForms32[] = {{kMiddle, 128, 128, 2, 61.f}, {kSmall, 64, 64, 2, 17.f}, {kThin, 16, 64, 3, 6.f}};
+template <typename TILES>
+Form best_form(uint32_t element_bytes, TILES tiles) {
+  const FormTime *const forms = element_bytes == 2 ? kForms16 : kForms32;
+  const uint64_t cus = device_info().num_cu;
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 3; ++i) {
+    uint64_t turns = (tiles(forms[i].height, forms[i].width) + cus - 1) / cus;
+    turns = turns < forms[i].share ? forms[i].share : turns;
+    const float time = forms[i].time * static_cast<float>(turns);
+    if (i == 0 || time < least) best = i, least = time;
+  }
+  return forms[best].form;
+}
+
 template <typename T, typename SHAPES>
 void choose_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
-  const uint32_t mean = d.rows / d.experts;
+  // (an expert's last tile is half full on average, and every expert that has rows has one)
+  const Form form = best_form(sizeof(T), [&](uint32_t height, uint32_t width) {
+    const uint64_t full = d.rows / height + d.experts / 2, least = d.experts < d.rows ? d.experts : d.rows;
+    return (full > least ? full : least) * div_up(d.out, width);
+  });
   if constexpr (sizeof(T) == 2) {
-    if (mean >= 192) return launch_product<T, typename SHAPES::Large>(target, stream, d, buffers);
+    if (form == kLarge) return launch_product<T, typename SHAPES::Large>(target, stream, d, buffers);
+  } else {
+    if (form == kThin) return launch_product<T, typename SHAPES::Thin>(target, stream, d, buffers);
   }
-  if (mean >= 48)
+  if (form == kMiddle)
     launch_product<T, typename SHAPES::Middle>(target, stream, d, buffers);
   else
     launch_product<T, typename SHAPES::Small>(target, stream, d, buffers);
@@ -727,25 +787,49 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
     choose_product<T, Staged>(target, stream, d, buffers);
 }
 
-template <typename T, typename S>
-void launch_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
-                     uint32_t n_left, uint32_t n_right, void **buffers) {
-  const uint64_t blocks = 8 * ((static_cast<uint64_t>(div_up(n_left, S::BM)) * div_up(n_right, S::BN) + 7) / 8) * d.experts;
-  if (refuse_grid(target, blocks) || !allow_lds(target, gradient_kernel<T, S>, S::kLdsBytes)) return;
-  hipLaunchKernelGGL((gradient_kernel<T, S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), S::kLdsBytes, stream,
-                     static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(buffers[2]),
-                     static_cast<T *>(buffers[3]), d.rows, d.experts, n_left, n_right);
-  check_launch(target);
+// The gradient's shape, and into how many parts an expert's rows are split where the tiles leave places on the card free: at
+// least 512 rows to a part on average (2 experts of 16,384 rows, 64 x 64 results: @SPLIT@).
+struct GradientPlan {
+  Form form;
+  uint32_t parts;
+};
+// (One plan whichever way the matrix is stored: the caller's scratch memory goes by it.)
+GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t experts, uint32_t inner, uint32_t out) {
+  const auto tiles = [&](uint32_t height, uint32_t width) {
+    return static_cast<uint64_t>(experts) * div_up(inner, height) * div_up(out, width);
+  };
+  GradientPlan p;
+  p.form = best_form(element_bytes, tiles);
+  if (p.form == kThin) p.form = kSmall;
+  const uint32_t side = p.form == kLarge ? 256 : p.form == kMiddle ? 128 : 64;
+  const uint64_t free = 2ull * device_info().num_cu / tiles(side, side), most = rows / experts / 512;
+  p.parts = static_cast<uint32_t>(free < most ? free : most);
+  if (p.parts < 1 || p.form == kLarge) p.parts = 1;
+  return p;
 }
 
-template <typename T, typename SHAPES>
-void choose_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
-                     uint32_t n_left, uint32_t n_right, void **buffers) {
-  if constexpr (sizeof(T) == 2) {
-    if (static_cast<uint64_t>(d.experts) * div_up(n_left, 256) * div_up(n_right, 256) >= 256)
-      return launch_gradient<T, typename SHAPES::Large>(target, stream, d, left, right, n_left, n_right, buffers);
+template <typename T, typename O, typename S>
+bool launch_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
+                     uint32_t n_left, uint32_t n_right, const void *indptr, O *out, uint32_t parts) {
+  const uint64_t blocks = 8 * ((static_cast<uint64_t>(div_up(n_left, S::BM)) * div_up(n_right, S::BN) + 7) / 8) * d.experts * parts;
+  // (threads of a launch are counted in 32 bits)
+  if (refuse_tiles(target, blocks, (1ull << 32) / S::kThreads) || !allow_lds(target, gradient_kernel<T, O, S>, S::kLdsBytes)) return false;
+  hipLaunchKernelGGL((gradient_kernel<T, O, S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), S::kLdsBytes, stream,
+                     static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(indptr), out,
+                     d.rows, d.experts, n_left, n_right, parts);
+  return check_launch(target);
+}
+
+template <typename T, typename O, typename SHAPES>
+bool choose_gradient(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, const void *left, const void *right,
+                     uint32_t n_left, uint32_t n_right, const void *indptr, O *out, const GradientPlan &plan) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, O>::value) {
+    if (plan.form == kLarge)
+      return launch_gradient<T, O, typename SHAPES::Large>(target, stream, d, left, right, n_left, n_right, indptr, out, plan.parts);
   }
-  launch_gradient<T, typename SHAPES::Middle>(target, stream, d, left, right, n_left, n_right, buffers);
+  if (plan.form == kMiddle)
+    return launch_gradient<T, O, typename SHAPES::Middle>(target, stream, d, left, right, n_left, n_right, indptr, out, plan.parts);
+  return launch_gradient<T, O, typename SHAPES::Small>(target, stream, d, left, right, n_left, n_right, indptr, out, plan.parts);
 }
 
 template <typename T>
@@ -756,15 +840,34 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
   const uint32_t n_left = out_major ? d.out : d.width, n_right = out_major ? d.width : d.out;
   const void *const left = buffers[out_major ? 1 : 0], *const right = buffers[out_major ? 0 : 1];
-  if (whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right))
-    choose_gradient<T, Direct>(target, stream, d, left, right, n_left, n_right, buffers);
-  else
-    choose_gradient<T, Staged>(target, stream, d, left, right, n_left, n_right, buffers);
+  const GradientPlan plan = gradient_plan(sizeof(T), d.rows, d.experts, d.width, d.out);
+  const bool direct = whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right);
+  const auto run = [&](auto *out) {
+    typedef std::remove_pointer_t<decltype(out)> O;
+    return direct ? choose_gradient<T, O, Direct>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan)
+                  : choose_gradient<T, O, Staged>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
+  };
+  if (plan.parts == 1) {
+    run(static_cast<T *>(buffers[3]));
+    return;
+  }
+  if (!run(static_cast<float *>(buffers[4]))) return;
+  const size_t n = static_cast<size_t>(d.experts) * n_left * n_right;
+  hipLaunchKernelGGL(join_kernel<T>, dim3(div_up(n, 256) < 4096 ? div_up(n, 256) : 4096), dim3(256), 0, stream,
+                     static_cast<const float *>(buffers[4]), static_cast<T *>(buffers[3]), n, plan.parts);
+  check_launch(target);
 }
 
 }  // namespace
 
 extern "C" {
+
+size_t bpl_expert_matmul_gradient_scratch_bytes(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
+                                                uint32_t element_bytes) {
+  if (experts == 0 || width == 0 || out_width == 0) return 0;
+  const GradientPlan plan = gradient_plan(element_bytes, rows, experts, width, out_width);
+  return plan.parts == 1 ? 0 : static_cast<size_t>(plan.parts) * experts * width * out_width * sizeof(float);
+}
 
 BPL_EXPERT_DEFINE(expert_matmul, matmul)
 BPL_EXPERT_DEFINE(expert_matmul_gradient, matmul_gradient)

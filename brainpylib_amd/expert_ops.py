@@ -359,7 +359,9 @@ class _ExpertMatmul(torch.autograd.Function):
       d_stored = torch.empty_like(stored)
       opaque = _lib.build_expert_descriptor(0, 0, stored.shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
                                             _OUT_MAJOR if ctx.out_major else 0)
-      _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct, indptr, d_stored], opaque)
+      scratch = torch.empty(_lib.expert_matmul_gradient_scratch_bytes(rows.shape[0], stored.shape[0], rows.shape[1], ct.shape[1],
+                                                                      rows.element_size()), dtype=torch.uint8, device=rows.device)
+      _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct, indptr, d_stored, scratch], opaque)
     sources = (given, rows, stored)
     return _first_order('expert_matmul', d_rows, *sources), _first_order('expert_matmul', d_stored, *sources), None, None
 

@@ -164,6 +164,9 @@ size_t bpl_build_expert_descriptor(uint32_t tokens, uint32_t per_token, uint32_t
                                    uint32_t out_width, uint32_t flags, char *out, size_t cap);
 /* Bytes of scratch memory that expert_sort of so many pairs takes as its last buffer. */
 size_t bpl_expert_sort_scratch_bytes(uint32_t pairs, uint32_t experts);
+/* The same for expert_matmul_gradient_T; element_bytes: of T. */
+size_t bpl_expert_matmul_gradient_scratch_bytes(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
+                                                uint32_t element_bytes);
 size_t bpl_build_event_csr_batching_descriptor(uint32_t n_row, uint32_t n_col, uint32_t batch_size,
                                                uint32_t values_batch, uint32_t indices_batch,
                                                uint32_t indptr_batch, uint32_t events_batch, uint32_t nnz,
@@ -615,7 +618,7 @@ BPL_TARGET(nonzero_double);
  *                          indptr int32[experts + 1], out T[rows][out]]
  *                          out[r] = rows[r] @ weight[e] for indptr[e] <= r < indptr[e + 1] (indptr[0] is taken as 0), zero
  *                          from indptr[experts] on; sums in float
- * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight]: rows_e^T @ d_out_e, zero for an expert
+ * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight, scratch]: rows_e^T @ d_out_e, zero for an expert
  *                          without rows.  (The gradient of the rows is expert_matmul with the weight's other storage.)
  * ---------------------------------------------------------------------------------------- */
 BPL_TARGET(expert_topk_float);

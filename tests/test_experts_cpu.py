@@ -43,6 +43,16 @@ def test_sort_scratch_is_for_long_lists_only():
   assert _lib.expert_sort_scratch_bytes(2 ** 31 - 1, 1024) < 1 << 26
 
 
+def test_gradient_scratch_is_the_parts_of_few_results():
+  size = _lib.expert_matmul_gradient_scratch_bytes
+  assert size(100, 8, 2048, 2048, 2) == 0 and size(0, 8, 64, 64, 4) == 0 and size(100_000, 4, 0, 64, 4) == 0
+  assert size(1 << 20, 64, 4096, 4096, 2) == 0
+  for width, out in ((64, 64), (30, 700), (700, 30), (1, 5), (5, 1)):
+    for element in (2, 4):
+      n = size(100_000, 2, width, out, element)
+      assert n > 0 and n % (2 * width * out * 4) == 0 and n <= 2 * width * out * 4 * 97
+
+
 @pytest.mark.parametrize("call, error", [
   (lambda: bpl.expert_topk(torch.zeros(2, 4, dtype=torch.float64), k=1), TypeError),
   (lambda: bpl.expert_topk(torch.zeros(2, 4, dtype=torch.int32), k=1), TypeError),

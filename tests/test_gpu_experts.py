@@ -276,6 +276,26 @@ def test_matmul(cuda, dtype, out_major, n, experts, inner, out):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, experts, inner, out", [(5000, 1, 64, 72), (9000, 3, 33, 50), (20_000, 2, 130, 64), (6000, 5, 8, 300)])
+def test_matmul_gradient_of_few_results_over_many_rows(cuda, dtype, n, experts, inner, out):
+  # an expert's rows are split into parts, and those added: the experts' numbers of rows are uneven, one has none
+  indptr = counts(n + out, n, experts, empty=0.0)
+  if experts > 2:
+    indptr[2] = indptr[1]
+  rows, ct = normal(1, n, inner, dtype=dtype), normal(2, n, out, dtype=dtype)
+  behind = int(indptr[-1])
+  rows[behind:], ct[behind:] = float("nan"), float("inf")
+  weight = torch.zeros(experts, inner, out, dtype=dtype)
+  want = plain.matmul_gradients(rows, weight, indptr, ct)[1]
+  size = plain.matmul_gradients(rows.abs(), weight, indptr, ct.abs())[1]
+  for out_major in (False, True):
+    stored = (weight.transpose(1, 2).contiguous() if out_major else weight).cuda().requires_grad_()
+    got = bpl.expert_matmul(rows.cuda(), stored.transpose(1, 2) if out_major else stored, indptr.cuda())
+    (d_stored,) = torch.autograd.grad(got, stored, ct.cuda())
+    check_sums(d_stored.transpose(1, 2) if out_major else d_stored, want, size, int((indptr[1:] - indptr[:-1]).max()) + 1, "d_weight")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_matmul_one_at_the_edges_of_the_tiles(cuda, dtype):
   # whole numbers, small enough that every product and sum is exact: equal, element for element
   for n in (15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257):
