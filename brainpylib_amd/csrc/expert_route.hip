@@ -258,39 +258,61 @@ void topk_gradient(const char *target, hipStream_t stream, void **buffers, const
 // (workgroup, expert) by one launch (none where one workgroup takes all), then every workgroup adds up the counts before
 // its own, scans the experts and ranks its pairs 64 at a time, in their order.  What is dropped counts as one more
 // expert behind the last.  No atomics but in counts, so the result never depends on an order.
+// Bound by the chain of its steps, not by bytes: 524,296 pairs over 256 experts @SORT@.
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / kWave;
-constexpr uint32_t kSortPairs = 4096;    // to a workgroup, at least
+constexpr uint32_t kSortPairs = 2048;  // to a workgroup, at least
+constexpr uint32_t kSortOne = 8192;    // so many pairs one workgroup takes alone
 constexpr uint32_t kSortMostGroups = 256;
+constexpr uint32_t kSortAtOnce = 4;    // steps of 64 pairs whose experts a wave requests together
 
 struct SortShape {
   uint32_t groups, pairs;  // workgroups, pairs to each (a multiple of kSortThreads)
 };
 SortShape sort_shape(uint32_t pairs) {
   SortShape s;
-  s.groups = pairs <= kSortPairs ? 1u : div_up(pairs, kSortPairs);
+  s.groups = pairs <= kSortOne ? 1u : div_up(pairs, kSortPairs);
   if (s.groups > kSortMostGroups) s.groups = kSortMostGroups;
   s.pairs = (div_up(pairs, s.groups) + kSortThreads - 1) / kSortThreads * kSortThreads;
   if (s.pairs == 0) s.pairs = kSortThreads;
   s.groups = pairs == 0 ? 1u : div_up(pairs, s.pairs);
   return s;
 }
+// A workgroup's row of counts: one for each expert and one for what is dropped, in whole quads.
+__host__ __device__ inline uint32_t sort_bins(uint32_t experts) { return (experts + 4u) / 4u * 4u; }
+
+// f(step, expert, whether there is a pair) for a wave's pairs from `first` on, 64 a step.
+template <typename FN>
+__device__ __forceinline__ void sort_steps(const uint32_t *__restrict__ chosen, uint64_t first, uint32_t part, uint32_t pairs,
+                                           uint32_t experts, FN f) {
+  const uint32_t lane = threadIdx.x % kWave;
+  for (uint32_t i0 = 0; i0 < part; i0 += kSortAtOnce * kWave) {
+    uint32_t e[kSortAtOnce];
+#pragma unroll
+    for (uint32_t j = 0; j < kSortAtOnce; ++j) {
+      const uint64_t p = first + i0 + j * kWave + lane;
+      e[j] = i0 + j * kWave < part && p < pairs ? chosen[p] : 0u;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kSortAtOnce; ++j) {
+      const uint64_t p = first + i0 + j * kWave + lane;
+      if (i0 + j * kWave < part) f(p, e[j] < experts ? e[j] : experts, p < pairs);
+    }
+  }
+}
 
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const uint32_t *__restrict__ chosen, uint32_t *__restrict__ counts,
                                                                   uint32_t pairs, uint32_t experts, uint32_t share) {
-  __shared__ uint32_t count[kMostExperts + 1];
-  for (uint32_t e = threadIdx.x; e <= experts; e += kSortThreads) count[e] = 0;
+  __shared__ uint32_t count[kMostExperts + 4];
+  const uint32_t bins = sort_bins(experts);
+  for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) count[e] = 0;
   __syncthreads();
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * share;
-  for (uint32_t i = threadIdx.x; i < share; i += kSortThreads) {
-    const uint64_t p = first + i;
-    if (p < pairs) {
-      const uint32_t e = chosen[p];
-      atomicAdd(&count[e < experts ? e : experts], 1u);
-    }
-  }
+  const uint32_t part = share / kSortWaves;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * share + threadIdx.x / kWave * part;
+  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t, uint32_t e, bool there) {
+    if (there) atomicAdd(&count[e], 1u);
+  });
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e <= experts; e += kSortThreads)
-    counts[static_cast<size_t>(blockIdx.x) * (experts + 1) + e] = count[e];
+  for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) counts[static_cast<size_t>(blockIdx.x) * bins + e] = count[e];
 }
 
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t *__restrict__ chosen, const uint32_t *__restrict__ counts,
@@ -300,7 +322,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
   // next[wave][expert]: first the wave's counts, then the place of its next pair of that expert
   extern __shared__ uint32_t lds[];
   uint32_t *const next = lds;
-  const uint32_t bins = experts + 1;
+  const uint32_t bins = sort_bins(experts);
   uint32_t *const total = next + kSortWaves * bins, *const before = total + bins;
   __shared__ uint32_t wave_total[kSortWaves];
   const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -309,41 +331,42 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
   uint32_t *const mine = next + wave * bins;
   const uint32_t part = share / kSortWaves;  // (a multiple of 64)
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * share + wave * part;
-  for (uint32_t i = lane; i < part; i += kWave) {
-    if (first + i < pairs) {
-      const uint32_t e = chosen[first + i];
-      atomicAdd(&mine[e < experts ? e : experts], 1u);
+  if (groups != 1) {
+    // four experts to a lane, lanes side by side; sets of them share the workgroups' counts
+    const uint32_t quads = bins / 4, sets = kSortThreads / quads, set = threadIdx.x / quads, quad = threadIdx.x % quads;
+    if (set < sets) {
+      uint4 all = make_uint4(0, 0, 0, 0), below = all;
+      const uint4 *const from = reinterpret_cast<const uint4 *>(counts) + quad;
+      // (a share to a set, its rows one after the other: eight requests under way)
+      const uint32_t rows = (groups + sets - 1) / sets, b0 = set * rows, b1 = b0 + rows < groups ? b0 + rows : groups;
+#pragma unroll 8
+      for (uint32_t b = b0; b < b1; ++b) {
+        const uint4 c = from[static_cast<size_t>(b) * quads];
+        const uint32_t mask = b < blockIdx.x ? 0xffffffffu : 0u;
+        all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+        below.x += c.x & mask, below.y += c.y & mask, below.z += c.z & mask, below.w += c.w & mask;
+      }
+      atomicAdd(&total[4 * quad], all.x), atomicAdd(&total[4 * quad + 1], all.y);
+      atomicAdd(&total[4 * quad + 2], all.z), atomicAdd(&total[4 * quad + 3], all.w);
+      atomicAdd(&before[4 * quad], below.x), atomicAdd(&before[4 * quad + 1], below.y);
+      atomicAdd(&before[4 * quad + 2], below.z), atomicAdd(&before[4 * quad + 3], below.w);
     }
   }
+  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t, uint32_t e, bool there) {
+    if (there) atomicAdd(&mine[e], 1u);
+  });
   __syncthreads();
   if (groups == 1) {
     for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) {
       uint32_t sum = 0;
+#pragma unroll
       for (uint32_t w = 0; w < kSortWaves; ++w) sum += next[w * bins + e];
       total[e] = sum;
     }
-  } else {
-    // lanes side by side take experts side by side; where there are fewer experts than threads, sets of threads share
-    // the workgroups' counts
-    const uint32_t stride = bins < kSortThreads ? bins : kSortThreads, sets = kSortThreads / stride;
-    const uint32_t set = threadIdx.x / stride;
-    if (set < sets) {
-      for (uint32_t e = threadIdx.x % stride; e < bins; e += stride) {
-        uint32_t all = 0, below = 0;
-#pragma unroll 8
-        for (uint32_t b = set; b < groups; b += sets) {
-          const uint32_t c = counts[static_cast<size_t>(b) * bins + e];
-          all += c;
-          below += b < blockIdx.x ? c : 0u;
-        }
-        atomicAdd(&total[e], all);
-        atomicAdd(&before[e], below);
-      }
-    }
+    __syncthreads();
   }
-  __syncthreads();
   // exclusive scan of the totals, consecutive experts to a thread
-  constexpr uint32_t kPer = (kMostExperts + 1 + kSortThreads - 1) / kSortThreads;
+  constexpr uint32_t kPer = (kMostExperts + 4 + kSortThreads - 1) / kSortThreads;
   uint32_t own[kPer], sum = 0;
 #pragma unroll
   for (uint32_t j = 0; j < kPer; ++j) {
@@ -355,35 +378,36 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
   if (lane == kWave - 1) wave_total[wave] = upto;
   __syncthreads();
   uint32_t start = upto - sum;
-  for (uint32_t w = 0; w < wave; ++w) start += wave_total[w];
+#pragma unroll
+  for (uint32_t w = 0; w < kSortWaves; ++w) start += w < wave ? wave_total[w] : 0u;
 #pragma unroll
   for (uint32_t j = 0; j < kPer; ++j) {
     const uint32_t e = threadIdx.x * kPer + j;
-    if (e < bins) {
-      if (blockIdx.x == 0) indptr[e] = start;
-      uint32_t at = start + before[e];
-      for (uint32_t w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = next[w * bins + e];
-        next[w * bins + e] = at;
-        at += c;
-      }
-    }
+    if (e < bins) before[e] += start;
+    if (e <= experts && blockIdx.x == 0) indptr[e] = start;
     start += own[j];
   }
   __syncthreads();
-  const uint32_t bits = 32u - __builtin_clz(bins);
+  for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) {
+    uint32_t c[kSortWaves], at = before[e];
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) c[w] = next[w * bins + e];
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) {
+      next[w * bins + e] = at;
+      at += c[w];
+    }
+  }
+  __syncthreads();
+  const uint32_t bits = 32u - __builtin_clz(experts);
   volatile uint32_t *const places = mine;
-  for (uint32_t i = 0; i < part; i += kWave) {
-    const uint64_t p = first + i + lane;
-    const bool active = p < pairs;
-    uint32_t e = active ? chosen[p] : 0u;
-    e = e < experts ? e : experts;
-    uint64_t same = __ballot(active);
+  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t p, uint32_t e, bool there) {
+    uint64_t same = __ballot(there);
     for (uint32_t b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((e >> b) & 1u);
       same &= (e >> b) & 1u ? set : ~set;
     }
-    if (active) {
+    if (there) {
       const uint32_t rank = __popcll(same & ((1ull << lane) - 1ull));
       const uint32_t at = places[e] + rank;
       // (a wave's LDS instructions are carried out in order: all lanes have read before the first of a kind adds)
@@ -394,7 +418,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
       order[at] = dropped ? kNone : static_cast<uint32_t>(p);
       position[p] = dropped ? kNone : at;
     }
-  }
+  });
 }
 
 void sort(const char *target, hipStream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
@@ -409,7 +433,7 @@ void sort(const char *target, hipStream_t stream, void **buffers, const char *op
                        s.pairs);
     if (!check_launch(target)) return;
   }
-  hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), (kSortWaves + 2) * (d.experts + 1) * 4, stream,
+  hipLaunchKernelGGL(sort_place_kernel, dim3(s.groups), dim3(kSortThreads), (kSortWaves + 2) * sort_bins(d.experts) * 4, stream,
                      chosen, counts, static_cast<uint32_t *>(buffers[1]), static_cast<uint32_t *>(buffers[2]),
                      static_cast<uint32_t *>(buffers[3]), pairs, d.experts, s.pairs, s.groups);
   check_launch(target);
@@ -674,7 +698,7 @@ extern "C" {
 
 size_t bpl_expert_sort_scratch_bytes(uint32_t pairs, uint32_t experts) {
   const SortShape s = sort_shape(pairs);
-  return s.groups > 1 ? static_cast<size_t>(s.groups) * (experts + 1) * sizeof(uint32_t) : 0;
+  return s.groups > 1 ? static_cast<size_t>(s.groups) * sort_bins(experts) * sizeof(uint32_t) : 0;
 }
 
 BPL_EXPERT_DEFINE(expert_topk, topk)
