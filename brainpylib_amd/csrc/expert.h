@@ -19,12 +19,14 @@ struct Piece {
 };
 
 // Elements col .. col + kElems - 1 of a row of `width`, zero beyond its end.  (The row may begin at any element: loads of
-// 16 bytes need no alignment here, and nothing beyond the row is touched.)
-template <typename T>
+// 16 bytes need no alignment here, and nothing beyond the row is touched.)  WHOLE: the row is known to end with a piece, so
+// that there is no other way to take.  ONCE: what is read once, and is to take no room in the caches from what is not.
+template <typename T, bool WHOLE = false, bool ONCE = false>
 __device__ __forceinline__ typename Piece<T>::type load_piece(const T *__restrict__ row, uint32_t col, uint32_t width) {
   typename Piece<T>::type v;
-  if (col + Piece<T>::kElems <= width) {
-    v = *reinterpret_cast<const typename Piece<T>::type *>(row + col);
+  if (WHOLE || col + Piece<T>::kElems <= width) {
+    const auto *const from = reinterpret_cast<const typename Piece<T>::type *>(row + col);
+    v = ONCE ? __builtin_nontemporal_load(from) : *from;
   } else {
 #pragma unroll
     for (uint32_t j = 0; j < Piece<T>::kElems; ++j) v[j] = col + j < width ? row[col + j] : static_cast<T>(0.f);
@@ -32,10 +34,15 @@ __device__ __forceinline__ typename Piece<T>::type load_piece(const T *__restric
   return v;
 }
 
-template <typename T>
+// PAST: past the caches, for results larger than they are (kept there, they only push out what is read again).
+template <typename T, bool WHOLE = false, bool PAST = false>
 __device__ __forceinline__ void store_piece(T *__restrict__ row, uint32_t col, uint32_t width, typename Piece<T>::type v) {
-  if (col + Piece<T>::kElems <= width) {
-    *reinterpret_cast<typename Piece<T>::type *>(row + col) = v;
+  if (WHOLE || col + Piece<T>::kElems <= width) {
+    auto *const to = reinterpret_cast<typename Piece<T>::type *>(row + col);
+    if (PAST)
+      __builtin_nontemporal_store(v, to);
+    else
+      *to = v;
   } else {
 #pragma unroll
     for (uint32_t j = 0; j < Piece<T>::kElems; ++j)

@@ -462,7 +462,7 @@ __device__ __forceinline__ Pair pair_of(const uint32_t *__restrict__ order, cons
 
 // Rows that no pair leads to are zero: the lanes of a wave look at a row each of the eight that it takes.
 constexpr uint32_t kZeroRows = 8;
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void zero_rows(const uint32_t *__restrict__ order, const uint32_t *__restrict__ position,
                                           T *__restrict__ rows, uint32_t pairs, uint32_t width, uint32_t unit) {
   const uint32_t lane = threadIdx.x % kWave;
@@ -480,11 +480,11 @@ __device__ __forceinline__ void zero_rows(const uint32_t *__restrict__ order, co
     const uint32_t j = __builtin_ctzll(left);
     left &= left - 1;
     T *const to = rows + (static_cast<size_t>(unit) * kZeroRows + j) * width;
-    for (uint32_t col = lane * Piece<T>::kElems; col < width; col += kWave * Piece<T>::kElems) store_piece<T>(to, col, width, zero);
+    for (uint32_t col = lane * Piece<T>::kElems; col < width; col += kWave * Piece<T>::kElems) store_piece<T, WHOLE>(to, col, width, zero);
   }
 }
 
-template <typename T>
+template <typename T, bool WHOLE, bool PAST>
 __global__ __launch_bounds__(256) void dispatch_kernel(const T *__restrict__ tokens, const uint32_t *__restrict__ order,
                                                        const uint32_t *__restrict__ position, T *__restrict__ rows,
                                                        uint32_t n, uint32_t k, uint32_t width, uint32_t chunks,
@@ -493,18 +493,18 @@ __global__ __launch_bounds__(256) void dispatch_kernel(const T *__restrict__ tok
   const uint64_t waves = static_cast<uint64_t>(gridDim.x) * (256 / kWave);
   for (uint64_t u = static_cast<uint64_t>(blockIdx.x) * (256 / kWave) + threadIdx.x / kWave; u < units + zero_units; u += waves) {
     if (u >= units) {
-      zero_rows<T>(order, position, rows, pairs, width, static_cast<uint32_t>(u - units));
+      zero_rows<T, WHOLE>(order, position, rows, pairs, width, static_cast<uint32_t>(u - units));
       continue;
     }
     const uint32_t t = static_cast<uint32_t>(u / chunks), chunk = static_cast<uint32_t>(u % chunks);
     const uint32_t col = (chunk * kWave + lane) * Piece<T>::kElems;
     const Pair mine = pair_of(order, position, t, lane, k, pairs);
     typename Piece<T>::type v{};
-    if (col < width) v = load_piece<T>(tokens + static_cast<size_t>(t) * width, col, width);
+    if (col < width) v = load_piece<T, WHOLE>(tokens + static_cast<size_t>(t) * width, col, width);
     const uint32_t row = mine.answered ? mine.row : kNone;
     for (uint32_t i = 0; i < k; ++i) {
       const uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(row), static_cast<int>(i)));
-      if (to != kNone && col < width) store_piece<T>(rows + static_cast<size_t>(to) * width, col, width, v);
+      if (to != kNone && col < width) store_piece<T, WHOLE, PAST>(rows + static_cast<size_t>(to) * width, col, width, v);
     }
   }
 }
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ rows
       for (uint32_t j = 0; j < kAhead; ++j) {
         if (i0 + j >= k) continue;
         const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine.row), static_cast<int>(i0 + j)));
-        if (at != kNone && col < width) v[j] = load_piece<T>(rows + static_cast<size_t>(at) * width, col, width);
+        if (at != kNone && col < width) v[j] = load_piece<T, false, true>(rows + static_cast<size_t>(at) * width, col, width);
       }
 #pragma unroll
       for (uint32_t j = 0; j < kAhead; ++j) {
@@ -556,21 +556,22 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *__restrict__ rows
 }
 
 // d_rows[position[t][i]] = weights[t][i] * ct[t];  d_weights[t][i] = <ct[t], rows[position[t][i]]>: a workgroup to a
-// token, eight of its pairs at a time.
-template <typename T>
+// token, four of its pairs at a time (eight hold 136 registers and leave three waves to a SIMD: 131,080 rows of 2,048
+// bfloat16 250 us, four 232, with stores past the caches 203).
+template <typename T, bool WHOLE, bool PAST>
 __global__ __launch_bounds__(256) void combine_gradient_kernel(const T *__restrict__ rows, const float *__restrict__ weights,
                                                                const uint32_t *__restrict__ order,
                                                                const uint32_t *__restrict__ position, const T *__restrict__ ct,
                                                                T *__restrict__ d_rows, float *__restrict__ d_weights, uint32_t n,
                                                                uint32_t k, uint32_t width, uint32_t zero_groups) {
-  constexpr uint32_t kElems = Piece<T>::kElems, kAtOnce = 8, kWaves = 256 / kWave;
+  constexpr uint32_t kElems = Piece<T>::kElems, kAtOnce = 4, kWaves = 256 / kWave;
   __shared__ float partial[kWaves][kAtOnce];
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, pairs = n * k;
   const uint32_t workers = gridDim.x - zero_groups;
   if (blockIdx.x >= workers) {
     const uint32_t units = (pairs + kZeroRows - 1) / kZeroRows;
     for (uint32_t u = (blockIdx.x - workers) * kWaves + wave; u < units; u += zero_groups * kWaves)
-      zero_rows<T>(order, position, d_rows, pairs, width, u);
+      zero_rows<T, WHOLE>(order, position, d_rows, pairs, width, u);
     return;
   }
   for (uint32_t t = blockIdx.x; t < n; t += workers) {
@@ -584,14 +585,14 @@ __global__ __launch_bounds__(256) void combine_gradient_kernel(const T *__restri
         const uint32_t col = base + threadIdx.x * kElems;
         const bool inside = col < width;  // (all lanes stay in the loop: each holds a pair that the others read)
         typename Piece<T>::type g{}, v[kAtOnce];
-        if (inside) g = load_piece<T>(from, col, width);
+        if (inside) g = load_piece<T, WHOLE>(from, col, width);
         if (d_weights != nullptr) {
 #pragma unroll
           for (uint32_t j = 0; j < kAtOnce; ++j) {
             v[j] = typename Piece<T>::type{};
             if (i0 + j >= k) continue;
             const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(row), static_cast<int>(i0 + j)));
-            if (at != kNone && inside) v[j] = load_piece<T>(rows + static_cast<size_t>(at) * width, col, width);
+            if (at != kNone && inside) v[j] = load_piece<T, WHOLE, true>(rows + static_cast<size_t>(at) * width, col, width);
           }
         }
 #pragma unroll
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(256) void combine_gradient_kernel(const T *__restri
             typename Piece<T>::type r;
 #pragma unroll
             for (uint32_t c = 0; c < kElems; ++c) r[c] = static_cast<T>(by * static_cast<float>(g[c]));
-            if (inside) store_piece<T>(d_rows + static_cast<size_t>(at) * width, col, width, r);
+            if (inside) store_piece<T, WHOLE, PAST>(d_rows + static_cast<size_t>(at) * width, col, width, r);
           }
           if (d_weights != nullptr) {
 #pragma unroll
@@ -631,6 +632,9 @@ __global__ __launch_bounds__(256) void combine_gradient_kernel(const T *__restri
   }
 }
 
+// Rows of 64 MB and more are stored past the caches: 131,080 rows of 2,048 bfloat16 114 -> 104 us there, 250 -> 203 us back.
+constexpr uint64_t kPastCaches = 64ull << 20;
+
 template <typename T>
 uint32_t chunks_of(uint32_t width) { return div_up(width, kWave * Piece<T>::kElems); }
 
@@ -642,7 +646,11 @@ void dispatch(const char *target, hipStream_t stream, void **buffers, const char
   if (pairs == 0 || d.width == 0) return;
   const uint32_t chunks = chunks_of<T>(d.width), zero_units = div_up(pairs, kZeroRows);
   const uint64_t units = static_cast<uint64_t>(d.tokens) * chunks;
-  hipLaunchKernelGGL(dispatch_kernel<T>, dim3(capped((units + zero_units + 3) / 4)), dim3(256), 0, stream,
+  // (lines that two waves write in part must meet in the cache: rows of 1,000 elements took 37 instead of 28 us)
+  const bool past = static_cast<uint64_t>(pairs) * d.width * sizeof(T) >= kPastCaches && d.width * sizeof(T) % 128 == 0 &&
+                    reinterpret_cast<uintptr_t>(buffers[3]) % 128 == 0;
+  const bool whole = d.width % Piece<T>::kElems == 0;
+  hipLaunchKernelGGL((past ? &dispatch_kernel<T, true, true> : whole ? &dispatch_kernel<T, true, false> : &dispatch_kernel<T, false, false>), dim3(capped((units + zero_units + 3) / 4)), dim3(256), 0, stream,
                      static_cast<const T *>(buffers[0]), static_cast<const uint32_t *>(buffers[1]),
                      static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.tokens, d.per_token,
                      d.width, chunks, units, zero_units);
@@ -685,7 +693,9 @@ void combine_gradient(const char *target, hipStream_t stream, void **buffers, co
   float *const d_weights = d.flags & BPL_EXPERT_D_WEIGHTS ? static_cast<float *>(buffers[6]) : nullptr;
   if (pairs == 0 || (d_rows == nullptr && d_weights == nullptr)) return;
   const uint32_t zero_groups = d_rows != nullptr ? capped(div_up(pairs, kZeroRows * 4)) : 0u;
-  hipLaunchKernelGGL(combine_gradient_kernel<T>, dim3(capped(d.tokens) + zero_groups), dim3(256), 0, stream,
+  const bool whole = d.width % Piece<T>::kElems == 0, past = static_cast<uint64_t>(pairs) * d.width * sizeof(T) >= kPastCaches;
+  hipLaunchKernelGGL((!whole ? &combine_gradient_kernel<T, false, false>
+                      : past ? &combine_gradient_kernel<T, true, true> : &combine_gradient_kernel<T, true, false>), dim3(capped(d.tokens) + zero_groups), dim3(256), 0, stream,
                      static_cast<const T *>(buffers[0]), static_cast<const float *>(buffers[1]),
                      static_cast<const uint32_t *>(buffers[2]), static_cast<const uint32_t *>(buffers[3]),
                      static_cast<const T *>(buffers[4]), d_rows, d_weights, d.tokens, d.per_token, d.width, zero_groups);
