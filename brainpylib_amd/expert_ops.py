@@ -17,7 +17,7 @@ none uses scratch memory that outlives it, so graphs share none.  Results do not
 import torch
 
 from . import _lib
-from ._tensors import as_tensor, device_of, has_tangent, is_index_dtype, keep_signature, to_device
+from ._tensors import as_tensor, device_of, has_tangent, is_index_dtype, to_device
 
 __all__ = ["expert_topk", "expert_sort", "expert_dispatch", "expert_combine", "expert_matmul"]
 
@@ -26,9 +26,17 @@ _NORMALIZE, _MASKED, _OUT_MAJOR, _D_ROWS, _D_WEIGHTS = 1, 2, 4, 8, 16  # BPL_EXP
 _MOST_EXPERTS, _MOST_PER_TOKEN, _MOST = 1024, 64, 2 ** 31 - 1
 
 
+def _current_device():
+  """The current device's index, replaced by torch's own function at its first call (``torch.cuda.current_device`` looks
+  first whether the device has been set up, which the tensors at hand say)."""
+  global _current_device
+  _current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
+  return _current_device()
+
+
 def _call(name, buffers, opaque):
   device = buffers[0].device
-  if device.index == torch.cuda.current_device():
+  if device.index == _current_device():
     _lib.custom_call(name, buffers, opaque)
   else:  # (a kernel is launched on the current device, whatever the stream's)
     with torch.cuda.device(device):
@@ -76,10 +84,12 @@ def _check_experts(n):
 
 def _differentiable(name, *tensors):
   """Whether a gradient is asked for; tangents are refused."""
+  wanted = False
   for t in tensors:
     if has_tangent(t):
       raise NotImplementedError(f'{name} has no forward-mode differentiation.')
-  return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    wanted = wanted or t.requires_grad
+  return wanted and torch.is_grad_enabled()
 
 
 class _FirstOrder(torch.autograd.Function):
@@ -118,22 +128,18 @@ def _topk(logits, mask, k, normalize):
   return weights, chosen
 
 
-@keep_signature
 class _ExpertTopk(torch.autograd.Function):
   """With w the weights, g their cotangent: normalized, the chosen logits' cotangents are w (g - sum w g) and the others'
   0; else, with p the softmax over all experts, p ([chosen] g - sum w g)."""
 
   @staticmethod
-  def forward(logits, mask, k, normalize):
-    return _topk(logits, mask, k, normalize)
-
-  @staticmethod
-  def setup_context(ctx, inputs, output):
-    logits, _, ctx.k, ctx.normalize = inputs
-    weights, chosen = output
+  def forward(ctx, logits, mask, k, normalize):
+    weights, chosen = _topk(logits, mask, k, normalize)
+    ctx.k, ctx.normalize = k, normalize
     ctx.mark_non_differentiable(chosen)
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(logits, weights, chosen)
+    return weights, chosen
 
   @staticmethod
   def backward(ctx, ct, _):
@@ -217,19 +223,14 @@ def _dispatch(tokens, order, position):
   return rows
 
 
-@keep_signature
 class _ExpertDispatch(torch.autograd.Function):
   """The cotangent of a token is the sum of its rows' cotangents."""
 
   @staticmethod
-  def forward(tokens, order, position):
-    return _dispatch(tokens, order, position)
-
-  @staticmethod
-  def setup_context(ctx, inputs, output):
-    _, order, position = inputs
+  def forward(ctx, tokens, order, position):
     ctx.save_for_backward(order, position)
     ctx.set_materialize_grads(False)
+    return _dispatch(tokens, order, position)
 
   @staticmethod
   def backward(ctx, ct):
@@ -267,18 +268,14 @@ def _combine(rows, weights, order, position):
   return out
 
 
-@keep_signature
 class _ExpertCombine(torch.autograd.Function):
   """The cotangent of a row is its token's times the pair's weight, that of the weight their inner product with the row."""
 
   @staticmethod
-  def forward(rows, weights, order, position):
-    return _combine(rows, weights, order, position)
-
-  @staticmethod
-  def setup_context(ctx, inputs, output):
-    ctx.save_for_backward(*inputs)
+  def forward(ctx, rows, weights, order, position):
+    ctx.save_for_backward(rows, weights, order, position)
     ctx.set_materialize_grads(False)
+    return _combine(rows, weights, order, position)
 
   @staticmethod
   def backward(ctx, ct):
@@ -332,19 +329,15 @@ def _matmul(rows, stored, indptr, out_major):
   return out
 
 
-@keep_signature
 class _ExpertMatmul(torch.autograd.Function):
   """The rows' cotangent is the product with the transposed weights, the weights' is rows_e^T @ ct_e for every expert."""
 
   @staticmethod
-  def forward(rows, stored, indptr, out_major):
-    return _matmul(rows, stored, indptr, out_major)
-
-  @staticmethod
-  def setup_context(ctx, inputs, output):
-    rows, stored, indptr, ctx.out_major = inputs
+  def forward(ctx, rows, stored, indptr, out_major):
+    ctx.out_major = out_major
     ctx.save_for_backward(rows, stored, indptr)
     ctx.set_materialize_grads(False)
+    return _matmul(rows, stored, indptr, out_major)
 
   @staticmethod
   def backward(ctx, ct):
