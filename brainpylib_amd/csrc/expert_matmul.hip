@@ -220,12 +220,19 @@ struct Shape {
 template <typename T, typename S>
 using Sums = typename Unit<T, S::kSide>::acc[S::kFragsM][S::kFragsN];
 
+typedef uint32_t quad32 __attribute__((ext_vector_type(4)));
+// Past the caches.  (As an instruction of its own: of a nontemporal store and a plain one that a branch chooses between, the
+// compiler makes one plain one.  The wait state is for what may overwrite the data's registers next.)
+__device__ __forceinline__ void store_past(void *to, quad32 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 0" ::"v"(to), "v"(v) : "memory");
+}
+
 // A wave's results to memory by way of a piece of LDS of its own, so that whole pieces of a row go side by side: a lane holds,
 // of row lane % kSide, 4 neighbouring columns at a time.  ROOM bytes hold kSide rows of so many of the wave's columns.  True: all of
 // the wave's results are there, and were stored in whole pieces.
 template <typename T, typename S, uint32_t ROOM, typename O>
 __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, uint32_t n0, uint32_t rows, uint32_t cols,
-                                           O *__restrict__ out, size_t out_stride, O *room) {
+                                           O *__restrict__ out, size_t out_stride, O *room, bool past) {
   constexpr uint32_t kElems = Piece<O>::kElems, kWide = S::BN / S::WN, kSide = S::kSide, kGroup = kWave / kSide * 4;
   constexpr uint32_t kCols = ROOM / kSide / sizeof(O) < kWide ? ROOM / kSide / sizeof(O) : kWide, kRow = kCols / kElems;
   static_assert(kCols % kGroup == 0 && kWide % kCols == 0 && (kRow & (kRow - 1)) == 0 && kWave % kRow == 0, "whole groups of columns");
@@ -255,7 +262,10 @@ __device__ __forceinline__ bool store_tile(const Sums<T, S> &sum, uint32_t m0, u
         return __builtin_bit_cast(typename Piece<O>::type, reinterpret_cast<const float4 *>(room)[row * kRow + (piece ^ (row & (kRow - 1)))]);
       };
       O *const to = out + (m0 + i * kSide + row0) * out_stride + n;
-      if (whole) {
+      if (whole && past) {
+#pragma unroll
+        for (uint32_t p = 0; p < kSide; p += kRows) store_past(to + p * out_stride, __builtin_bit_cast(quad32, held(p + row0)));
+      } else if (whole) {
 #pragma unroll
         for (uint32_t p = 0; p < kSide; p += kRows) *reinterpret_cast<typename Piece<O>::type *>(to + p * out_stride) = held(p + row0);
       } else {
@@ -317,7 +327,7 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     __syncthreads();
   }
   store_tile<T, S, S::kRoom, O>(sum, m0, n0, rows, cols, out, out_stride,
-                             reinterpret_cast<O *>(buffer) + wave * (S::kRoom / sizeof(O)));
+                             reinterpret_cast<O *>(buffer) + wave * (S::kRoom / sizeof(O)), false);
 }
 
 // ---- the same, with loads that go straight to LDS -----------------------------------------------------------------
@@ -396,10 +406,10 @@ struct Job {
   uint32_t rows, cols, depth;
 };
 
-// job(n, &j): the workgroup's n-th tile; false: there are no more.
+// jobs(at, &j): the workgroup's next tile from its place `at` on, which begins at 0; false: there are no more.
 template <typename T, typename O, bool A_ACROSS, bool B_ACROSS, typename S, typename JOBS>
 __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_stride, uint32_t b_stride, size_t out_stride,
-                                                float4 *lds) {
+                                                float4 *lds, bool past) {
   constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = S::kSteps, kSide = S::kSide, kRing = S::kStages;
   constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
   static_assert((kSteps == 4 || kSteps == 2) && (kRing & (kRing - 1)) == 0 && kRing >= 2, "what work() goes by");
@@ -413,12 +423,12 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kStageK<T>;
   const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
 
-  // what is filled: tile `filling`, from its stage `left` of `to_fill` on; `filled` and `done` count the stream's stages
+  // what is filled: the tile before `filling`, of which `depth_left` of k is left; `filled` and `done` count the stream's stages
   Job<T, O> from;
   LoaderA load_a;
   LoaderB load_b;
   uint32_t filling = 0, depth_left = 0, filled = 0, done = 0;
-  bool more = jobs(0, &from);
+  bool more = jobs(filling, &from);
   const auto begin = [&] {
     load_a.begin(from.rows, a_stride);
     load_b.begin(from.cols, b_stride);
@@ -440,7 +450,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   };
   const auto next_job = [&] {  // the next tile that has anything to fill
     while (more && depth_left == 0) {
-      more = jobs(++filling, &from);
+      more = jobs(filling, &from);
       if (more) begin();
     }
   };
@@ -530,7 +540,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
 #pragma unroll
   for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
   Job<T, O> now;
-  for (uint32_t n = 0; jobs(n, &now); ++n) {
+  for (uint32_t at = 0; jobs(at, &now);) {
     uint32_t left = (now.depth + kStageK<T> - 1) / kStageK<T>;
     while (left != 0) {
       next_job();
@@ -544,7 +554,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
       }
     }
     after = store_tile<T, S, S::kRoom, O>(sum, m0, n0, now.rows, now.cols, now.out, out_stride,
-                                       reinterpret_cast<O *>(buffer + kRing * (kA + kB)) + wave * (S::kRoom / sizeof(O)));
+                                       reinterpret_cast<O *>(buffer + kRing * (kA + kB)) + wave * (S::kRoom / sizeof(O)), past);
 #pragma unroll
     for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
@@ -580,39 +590,58 @@ __device__ __forceinline__ void zero_from(T *__restrict__ out, uint32_t first, u
   }
 }
 
-template <typename T, bool OUT_MAJOR, typename S>
+// Tiles are counted in those of `COARSE`.  S = COARSE takes all of them, or, `split` (in workgroups that the card holds at once),
+// as many as fill the card a whole number of times, if those left over fill it at most half; a second launch with a smaller S
+// then takes the smaller tiles of what is left over, on all of the card.
+template <typename T, bool OUT_MAJOR, typename S, typename COARSE>
 __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
                                                               const uint32_t *__restrict__ indptr, T *__restrict__ out,
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
-                                                              uint32_t cols) {
+                                                              uint32_t cols, uint32_t split, bool past) {
+  constexpr bool kRest = !std::is_same<S, COARSE>::value;
+  constexpr uint32_t kDown = COARSE::BM / S::BM, kAcross = COARSE::BN / S::BN;
   extern __shared__ float4 lds[];
   __shared__ TileTable table;
-  const uint32_t across = (cols + S::BN - 1) / S::BN;
-  const uint32_t total = table.build<S::kThreads>(indptr, experts, n_rows, S::BM);
-  const Turn turn = turn_of(static_cast<uint64_t>(total) * across);
-  const auto jobs = [&](uint32_t n, Job<T, T> *j) {
-    const uint32_t index = turn.index + n * turn.step;
-    if (index >= turn.end) return false;
-    const uint32_t down = uniform(index / across), col0 = (index - down * across) * S::BN;
-    const Tile tile = table.find(indptr, down, experts, n_rows, S::BM);
-    const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
-    j->a = uniform(rows + static_cast<size_t>(tile.first) * inner);
-    j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
-    j->out = out + static_cast<size_t>(tile.first) * cols + col0;
-    j->rows = tile.end - tile.first;
-    j->cols = cols - col0 < S::BN ? cols - col0 : S::BN;
-    j->depth = inner;
-    return true;
+  const uint32_t across = (cols + COARSE::BN - 1) / COARSE::BN;
+  const uint32_t total = table.build<S::kThreads>(indptr, experts, n_rows, COARSE::BM);
+  const uint64_t tiles = static_cast<uint64_t>(total) * across;
+  uint32_t rest = split != 0 ? static_cast<uint32_t>(tiles % split) : 0u;
+  if (rest > split / 2) rest = 0;
+  const Turn turn = turn_of(kRest ? static_cast<uint64_t>(rest) * (kDown * kAcross) : tiles - rest);
+  const auto jobs = [&](uint32_t &at, Job<T, T> *j) {
+    for (;;) {
+      uint32_t index = turn.index + at * turn.step, in = 0;
+      if (index >= turn.end) return false;
+      ++at;
+      if (kRest) {
+        in = index % (kDown * kAcross);
+        index = static_cast<uint32_t>(tiles - rest) + index / (kDown * kAcross);
+      }
+      const uint32_t down = uniform(index / across);
+      const uint32_t col0 = (index - down * across) * COARSE::BN + in % kAcross * S::BN;
+      const Tile tile = table.find(indptr, down, experts, n_rows, COARSE::BM);
+      const uint32_t first = tile.first + in / kAcross * S::BM;
+      if (kRest && (first >= tile.end || col0 >= cols)) continue;  // (beyond the tile's rows or columns)
+      const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
+      j->a = uniform(rows + static_cast<size_t>(first) * inner);
+      j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
+      j->out = out + static_cast<size_t>(first) * cols + col0;
+      j->rows = tile.end - first < S::BM ? tile.end - first : S::BM;
+      j->cols = cols - col0 < S::BN ? cols - col0 : S::BN;
+      j->depth = inner;
+      return true;
+    }
   };
   if constexpr (S::kStages != 0) {
-    stream_products<T, T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds);
+    stream_products<T, T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds, past);
   } else {
     Job<T, T> j;
-    for (uint32_t n = 0; jobs(n, &j); ++n) {
+    for (uint32_t at = 0; jobs(at, &j);) {
       tile_product<T, false, !OUT_MAJOR, S, T>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, inner, j.out, cols, lds);
       __syncthreads();
     }
   }
+  if (kRest) return;
   const uint32_t behind = indptr[experts];
   zero_from(out, behind < n_rows ? behind : n_rows, n_rows, cols, S::kThreads);
 }
@@ -624,24 +653,39 @@ template <typename T, typename O, typename S>
 __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
                                                                const uint32_t *__restrict__ indptr, O *__restrict__ d_weight,
                                                                uint32_t n_rows, uint32_t experts, uint32_t n_left,
-                                                               uint32_t n_right, uint32_t parts) {
+                                                               uint32_t n_right, uint32_t parts, bool past) {
   extern __shared__ float4 lds[];
   const uint32_t down = (n_left + S::BM - 1) / S::BM, across = (n_right + S::BN - 1) / S::BN;
   // An eighth of every expert's tiles to an XCD, neighbouring ones: the XCDs' work is the same however long the experts are.
+  // Of up to 64 experts the longest come first, so that what ends last is short.
   const uint32_t tiles = down * across, share = (tiles + 7) / 8;
-  const auto jobs = [&](uint32_t n, Job<T, O> *j) {
-    const uint32_t which = uniform(blockIdx.x / 8 / share), expert = uniform(which / parts), part = which - expert * parts;
-    const uint32_t in = (blockIdx.x + which * tiles) % 8 * share + blockIdx.x / 8 % share;
-    if (n != 0 || in >= tiles) return false;
-    const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
-    uint2 range = rows_of(indptr, expert, experts, n_rows);
-    if (parts != 1) {  // whole stages to a part
-      const uint32_t length = ((range.y - range.x + parts - 1) / parts + kDepth<T> - 1) / kDepth<T> * kDepth<T>;
-      const uint64_t from = static_cast<uint64_t>(range.x) + static_cast<uint64_t>(length) * part;
-      range.x = from < range.y ? static_cast<uint32_t>(from) : range.y;
-      range.y = range.y - range.x < length ? range.y : range.x + length;
+  const uint32_t which = uniform(blockIdx.x / 8 / share), part = which % parts;
+  const uint32_t in = (blockIdx.x + which * tiles) % 8 * share + blockIdx.x / 8 % share;
+  if (in >= tiles) return;
+  uint32_t expert = which / parts;
+  if (experts <= kWave) {
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint2 r = lane < experts ? rows_of(indptr, lane, experts, n_rows) : make_uint2(0, 0);
+    const uint32_t length = r.y - r.x;
+    uint32_t before = 0;
+    for (uint32_t e = 0; e < experts; ++e) {
+      const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(length), static_cast<int>(e)));
+      before += other > length || (other == length && e < lane) ? 1u : 0u;
     }
-    range = make_uint2(uniform(range.x), uniform(range.y));
+    expert = __builtin_ctzll(__ballot(lane < experts && before == expert));
+  }
+  expert = uniform(expert);
+  uint2 range = rows_of(indptr, expert, experts, n_rows);
+  if (parts != 1) {  // whole stages to a part
+    const uint32_t length = ((range.y - range.x + parts - 1) / parts + kDepth<T> - 1) / kDepth<T> * kDepth<T>;
+    const uint64_t from = static_cast<uint64_t>(range.x) + static_cast<uint64_t>(length) * part;
+    range.x = from < range.y ? static_cast<uint32_t>(from) : range.y;
+    range.y = range.y - range.x < length ? range.y : range.x + length;
+  }
+  range = make_uint2(uniform(range.x), uniform(range.y));
+  const uint32_t p0 = uniform(in / across) * S::BM, q0 = uniform(in % across) * S::BN;
+  const auto jobs = [&](uint32_t &at, Job<T, O> *j) {
+    if (at++ != 0) return false;
     j->a = uniform(left + static_cast<size_t>(range.x) * n_left + p0);
     j->b = uniform(right + static_cast<size_t>(range.x) * n_right + q0);
     j->out = d_weight + ((static_cast<size_t>(part) * experts + expert) * n_left + p0) * n_right + q0;
@@ -651,10 +695,10 @@ __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restri
     return true;
   };
   if constexpr (S::kStages != 0) {
-    stream_products<T, O, true, true, S>(jobs, n_left, n_right, n_right, lds);
+    stream_products<T, O, true, true, S>(jobs, n_left, n_right, n_right, lds, past);
   } else {
     Job<T, O> j;
-    for (uint32_t n = 0; jobs(n, &j); ++n) {
+    for (uint32_t at = 0; jobs(at, &j);) {
       tile_product<T, true, true, S, O>(j.a, j.rows, n_left, j.b, j.cols, n_right, j.depth, j.out, n_right, lds);
       __syncthreads();
     }
@@ -694,6 +738,13 @@ bool whole_pieces(const void *p, uint32_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % Piece<T>::kElems == 0 && stride < (1u << 20);
 }
 
+// Results of 64 MB and more in whole lines are stored past the caches (32,768 rows, 8 experts of 2,048 x 2,048, bfloat16: 262 ->
+// 241 us out-major, 248 -> 229 us; the gradient of such weights 240 -> 232).
+bool past_caches(const void *out, uint64_t rows, uint32_t cols, uint32_t element_bytes) {
+  const uint64_t line = static_cast<uint64_t>(cols) * element_bytes;
+  return rows * line >= 64ull << 20 && line % 128 == 0 && reinterpret_cast<uintptr_t>(out) % 128 == 0;
+}
+
 // Shapes for operands in whole pieces, and for others
 struct Direct {
   using Large = Shape<256, 256, 2, 2, 32, 2>;
@@ -708,25 +759,27 @@ struct Staged {
   using Thin = Shape<16, 64, 1, 2, 16, 0>;
 };
 
-template <typename T, typename S>
-void launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
-  const uint64_t tiles = most_tiles(d.rows, d.experts, S::BM) * div_up(d.out, S::BN);
-  if (refuse_tiles(target, tiles, 1ull << 32)) return;
+// `split`: whether what is left over of COARSE's tiles, when they have filled the card, is given to S.
+template <typename T, typename S, typename COARSE = S>
+bool launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers, bool split = false) {
+  constexpr uint32_t kDown = COARSE::BM / S::BM * (COARSE::BN / S::BN);
+  const uint64_t tiles = most_tiles(d.rows, d.experts, COARSE::BM) * div_up(d.out, COARSE::BN) * kDown;
+  if (refuse_tiles(target, tiles, 1ull << 32)) return false;
   // one workgroup to each place that the LDS leaves
-  const uint64_t places = static_cast<uint64_t>(device_info().num_cu) * (160u * 1024u / (S::kLdsBytes + sizeof(TileTable) + 1024u));
+  const auto held = [](uint32_t lds_bytes) {
+    return static_cast<uint32_t>(device_info().num_cu) * (160u * 1024u / (lds_bytes + static_cast<uint32_t>(sizeof(TileTable)) + 1024u));
+  };
+  const uint64_t places = held(S::kLdsBytes);
   const unsigned grid = static_cast<unsigned>(((tiles < places ? tiles : places) + 7) / 8 * 8);
   const auto launch = [&](auto *kernel) {
-    if (!allow_lds(target, kernel, S::kLdsBytes)) return;
+    if (!allow_lds(target, kernel, S::kLdsBytes)) return false;
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLdsBytes, stream,
                        static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
                        static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
-                       d.out);
-    check_launch(target);
+                       d.out, split ? held(COARSE::kLdsBytes) : 0u, past_caches(buffers[3], d.rows, d.out, sizeof(T)));
+    return check_launch(target);
   };
-  if (d.flags & BPL_EXPERT_OUT_MAJOR)
-    launch(product_kernel<T, true, S>);
-  else
-    launch(product_kernel<T, false, S>);
+  return d.flags & BPL_EXPERT_OUT_MAJOR ? launch(product_kernel<T, true, S, COARSE>) : launch(product_kernel<T, false, S, COARSE>);
 }
 
 // Which shape: the least time by the tiles that a CU works through one after the other (those that share it, at least) and a
@@ -743,15 +796,16 @@ struct FormTime {
 constexpr FormTime kForms16[] = {{kLarge, 256, 256, 1, 60.f}, {kMiddle, 128, 128, 2, 19.f}, {kSmall, 64, 64, 2, 8.5f}};
 constexpr FormTime kForms32[] = {{kMiddle, 128, 128, 2, 61.f}, {kSmall, 64, 64, 2, 17.f}, {kThin, 16, 64, 3, 6.f}};
 template <typename TILES>
-Form best_form(uint32_t element_bytes, TILES tiles) {
+Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
   const FormTime *const forms = element_bytes == 2 ? kForms16 : kForms32;
   const uint64_t cus = device_info().num_cu;
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 3; ++i) {
-    uint64_t turns = (tiles(forms[i].height, forms[i].width) + cus - 1) / cus;
-    turns = turns < forms[i].share ? forms[i].share : turns;
-    const float time = forms[i].time * static_cast<float>(turns);
+    const uint64_t n = tiles(forms[i].height, forms[i].width), held = cus * forms[i].share;
+    float turns = static_cast<float>((n + held - 1) / held * forms[i].share);
+    if (split && forms[i].form == kLarge && n % held != 0 && n % held <= held / 2) turns -= 0.35f;
+    const float time = forms[i].time * turns;
     if (i == 0 || time < least) best = i, least = time;
   }
   return forms[best].form;
@@ -760,14 +814,24 @@ Form best_form(uint32_t element_bytes, TILES tiles) {
 template <typename T, typename SHAPES>
 void choose_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
   // (an expert's last tile is half full on average, and every expert that has rows has one)
-  const Form form = best_form(sizeof(T), [&](uint32_t height, uint32_t width) {
+  const Form form = best_form(sizeof(T), d.width >= 512, [&](uint32_t height, uint32_t width) {
     const uint64_t full = d.rows / height + d.experts / 2, least = d.experts < d.rows ? d.experts : d.rows;
     return (full > least ? full : least) * div_up(d.out, width);
   });
   if constexpr (sizeof(T) == 2) {
-    if (form == kLarge) return launch_product<T, typename SHAPES::Large>(target, stream, d, buffers);
+    if (form == kLarge) {
+      // A tile that is left over takes a whole turn of the card, 60 us at an inner dimension of 2,048, in quarters 20 to
+      // 40; below 512 of it the second launch costs what that saves.
+      const bool split = d.width >= 512;
+      if (launch_product<T, typename SHAPES::Large>(target, stream, d, buffers, split) && split)
+        launch_product<T, typename SHAPES::Middle, typename SHAPES::Large>(target, stream, d, buffers, true);
+      return;
+    }
   } else {
-    if (form == kThin) return launch_product<T, typename SHAPES::Thin>(target, stream, d, buffers);
+    if (form == kThin) {
+      launch_product<T, typename SHAPES::Thin>(target, stream, d, buffers);
+      return;
+    }
   }
   if (form == kMiddle)
     launch_product<T, typename SHAPES::Middle>(target, stream, d, buffers);
@@ -799,7 +863,7 @@ GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t exper
     return static_cast<uint64_t>(experts) * div_up(inner, height) * div_up(out, width);
   };
   GradientPlan p;
-  p.form = best_form(element_bytes, tiles);
+  p.form = best_form(element_bytes, false, tiles);
   if (p.form == kThin) p.form = kSmall;
   const uint32_t side = p.form == kLarge ? 256 : p.form == kMiddle ? 128 : 64;
   const uint64_t free = 2ull * device_info().num_cu / tiles(side, side), most = rows / experts / 512;
@@ -816,7 +880,8 @@ bool launch_gradient(const char *target, hipStream_t stream, const bpl_expert_de
   if (refuse_tiles(target, blocks, (1ull << 32) / S::kThreads) || !allow_lds(target, gradient_kernel<T, O, S>, S::kLdsBytes)) return false;
   hipLaunchKernelGGL((gradient_kernel<T, O, S>), dim3(static_cast<unsigned>(blocks)), dim3(S::kThreads), S::kLdsBytes, stream,
                      static_cast<const T *>(left), static_cast<const T *>(right), static_cast<const uint32_t *>(indptr), out,
-                     d.rows, d.experts, n_left, n_right, parts);
+                     d.rows, d.experts, n_left, n_right, parts,
+                     past_caches(out, static_cast<uint64_t>(d.experts) * n_left * parts, n_right, sizeof(O)));
   return check_launch(target);
 }
 

@@ -275,6 +275,51 @@ def test_matmul(cuda, dtype, out_major, n, experts, inner, out):
   check_sums(d_weight, want[1], size[1], int((indptr[1:] - indptr[:-1]).max()) + 1, "d_weight")
 
 
+@pytest.mark.parametrize("dtype, out_major, n, experts, inner, out", [
+  (torch.bfloat16, True, 20_000, 4, 520, 1024), (torch.float16, False, 20_100, 5, 512, 1000), (torch.bfloat16, False, 18_000, 3, 517, 1031),
+  (torch.float32, True, 9000, 3, 130, 520), (torch.bfloat16, True, 9000, 30, 96, 520)])
+def test_matmul_of_many_tiles(cuda, dtype, out_major, n, experts, inner, out):
+  # more tiles than the card holds: the largest ones and what is left over of them, and the middle ones
+  indptr = counts(n, n, experts)
+  rows, ct, weight = normal(1, n, inner, dtype=dtype), normal(2, n, out, dtype=dtype), normal(3, experts, inner, out, dtype=dtype)
+  behind = int(indptr[-1])
+  rows[behind:], ct[behind:] = float("nan"), float("nan")
+  given = rows.cuda().requires_grad_()
+  stored = (weight.transpose(1, 2).contiguous() if out_major else weight).cuda().requires_grad_()
+  got = bpl.expert_matmul(given, stored.transpose(1, 2) if out_major else stored, indptr.cuda())
+  check_sums(got, plain.matmul(rows, weight, indptr), plain.matmul(rows.abs(), weight.abs(), indptr), inner, "out")
+  assert (got[behind:] == 0).all()
+  d_rows, d_stored = torch.autograd.grad(got, (given, stored), ct.cuda())
+  want, size = plain.matmul_gradients(rows, weight, indptr, ct), plain.matmul_gradients(rows.abs(), weight.abs(), indptr, ct.abs())
+  check_sums(d_rows, want[0], size[0], out, "d_rows")
+  d_weight = d_stored.transpose(1, 2) if out_major else d_stored
+  check_sums(d_weight, want[1], size[1], int((indptr[1:] - indptr[:-1]).max()) + 1, "d_weight")
+
+
+def test_results_that_are_stored_past_the_caches(cuda):
+  # more than 64 MB in whole lines: products, rows to the experts and the gradients
+  indptr = torch.tensor([0, 20_000, 20_000, 33_000], dtype=torch.int32)
+  g = torch.Generator().manual_seed(0)
+  rows = torch.randint(-2, 3, (34_000, 64), generator=g).to(torch.bfloat16)
+  weight = torch.randint(-1, 2, (3, 64, 1024), generator=g).to(torch.bfloat16)
+  got = bpl.expert_matmul(rows.cuda(), weight.cuda(), indptr.cuda())
+  want = torch.cat([rows[:20_000].float().cuda() @ weight[0].float().cuda(), rows[20_000:33_000].float().cuda() @ weight[2].float().cuda(),
+                    torch.zeros(1000, 1024, device="cuda")])
+  assert torch.equal(got.float(), want)  # (whole numbers below 256)
+  chosen = torch.from_numpy(choices(5, 4099, 8, 16)).cuda()
+  _, order, position = bpl.expert_sort(chosen, num_experts=16)
+  x = normal(1, 4099, 1088, dtype=torch.bfloat16).cuda()
+  sent = bpl.expert_dispatch(x, order, position)
+  live = order >= 0
+  assert torch.equal(sent, torch.where(live[:, None], x[order.clamp(min=0).long() // 8], 0.0))
+  by = normal(2, 4099, 8).cuda()
+  given = sent.clone().requires_grad_()
+  (d_rows,) = torch.autograd.grad(bpl.expert_combine(given, by, order, position), given, x)
+  at = order.clamp(min=0).long()
+  exact = torch.where(live[:, None], by.double().reshape(-1)[at][:, None] * x.double()[at // 8], 0.0)
+  check_sums(d_rows, exact.cpu(), exact.abs().cpu(), 1, "d_rows")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n, experts, inner, out", [(5000, 1, 64, 72), (9000, 3, 33, 50), (20_000, 2, 130, 64), (6000, 5, 8, 300)])
 def test_matmul_gradient_of_few_results_over_many_rows(cuda, dtype, n, experts, inner, out):
