@@ -51,8 +51,9 @@ def lib():
                  "bpl_build_nonzero_descriptor", "bpl_build_jitconn_prob_homo_descriptor",
                  "bpl_build_jitconn_prob_uniform_descriptor", "bpl_build_jitconn_prob_normal_descriptor",
                  "bpl_build_matmat_jit_prob_descriptor1", "bpl_build_expert_descriptor",
-                 "bpl_expert_sort_scratch_bytes", "bpl_expert_matmul_gradient_scratch_bytes"):
+                 "bpl_expert_sort_scratch_bytes"):
       getattr(l, name).restype = ctypes.c_size_t
+    l.bpl_expert_matmul_gradient_parts.restype = ctypes.c_uint32
     _lib = l
   return _lib
 
@@ -239,7 +240,6 @@ def expert_sort_scratch_bytes(pairs, experts):
   return lib().bpl_expert_sort_scratch_bytes(ctypes.c_uint32(pairs), ctypes.c_uint32(experts))
 
 
-@functools.lru_cache(maxsize=256)
-def expert_matmul_gradient_scratch_bytes(rows, experts, width, out_width, element_bytes):
+def expert_matmul_gradient_parts(rows, experts, width, out_width, element_bytes):
   u = ctypes.c_uint32
-  return lib().bpl_expert_matmul_gradient_scratch_bytes(u(rows), u(experts), u(width), u(out_width), u(element_bytes))
+  return lib().bpl_expert_matmul_gradient_parts(u(rows), u(experts), u(width), u(out_width), u(element_bytes))

@@ -85,7 +85,9 @@ struct TileTable {
     const uint32_t fine = __popcll(__ballot(lane < 16 && e < experts && start[e < experts ? e : 0] <= index));
     const uint32_t expert = uniform((coarse - 1) * 16 + fine - 1);
     const uint2 r = rows_of(indptr, expert, experts, rows);
-    const uint32_t first = uniform(r.x) + (index - uniform(start[expert])) * height, end = uniform(r.y);
+    // (of an indptr that is none, more tiles than 32 bits count may leave one beyond the rows: it is empty)
+    const uint64_t from = uniform(r.x) + static_cast<uint64_t>(index - uniform(start[expert])) * height;
+    const uint32_t end = uniform(r.y), first = from < end ? static_cast<uint32_t>(from) : end;
     return Tile{expert, first, end - first < height ? end : first + height};
   }
 };
@@ -621,7 +623,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
       const uint32_t col0 = (index - down * across) * COARSE::BN + in % kAcross * S::BN;
       const Tile tile = table.find(indptr, down, experts, n_rows, COARSE::BM);
       const uint32_t first = tile.first + in / kAcross * S::BM;
-      if (kRest && (first >= tile.end || col0 >= cols)) continue;  // (beyond the tile's rows or columns)
+      if (first >= tile.end || col0 >= cols) continue;  // (a quarter beyond the tile's rows or columns)
       const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
       j->a = uniform(rows + static_cast<size_t>(first) * inner);
       j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
@@ -764,7 +766,7 @@ template <typename T, typename S, typename COARSE = S>
 bool launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers, bool split = false) {
   constexpr uint32_t kDown = COARSE::BM / S::BM * (COARSE::BN / S::BN);
   const uint64_t tiles = most_tiles(d.rows, d.experts, COARSE::BM) * div_up(d.out, COARSE::BN) * kDown;
-  if (refuse_tiles(target, tiles, 1ull << 32)) return false;
+  if (refuse_tiles(target, tiles, 1ull << 31)) return false;
   // one workgroup to each place that the LDS leaves
   const auto held = [](uint32_t lds_bytes) {
     return static_cast<uint32_t>(device_info().num_cu) * (160u * 1024u / (lds_bytes + static_cast<uint32_t>(sizeof(TileTable)) + 1024u));
@@ -852,12 +854,12 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
 }
 
 // The gradient's shape, and into how many parts an expert's rows are split where the tiles leave places on the card free: at
-// least 512 rows to a part on average (2 experts of 16,384 rows, 64 x 64 results: @SPLIT@).
+// least 512 rows to a part on average (2 experts of 16,384 rows, 64 x 64 results: @SPLIT@).  How many parts there are is the
+// caller's, who brings the room for them; the shape is chosen here.
 struct GradientPlan {
   Form form;
   uint32_t parts;
 };
-// (One plan whichever way the matrix is stored: the caller's scratch memory goes by it.)
 GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t experts, uint32_t inner, uint32_t out) {
   const auto tiles = [&](uint32_t height, uint32_t width) {
     return static_cast<uint64_t>(experts) * div_up(inner, height) * div_up(out, width);
@@ -867,8 +869,8 @@ GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t exper
   if (p.form == kThin) p.form = kSmall;
   const uint32_t side = p.form == kLarge ? 256 : p.form == kMiddle ? 128 : 64;
   const uint64_t free = 2ull * device_info().num_cu / tiles(side, side), most = rows / experts / 512;
-  p.parts = static_cast<uint32_t>(free < most ? free : most);
-  if (p.parts < 1 || p.form == kLarge) p.parts = 1;
+  const uint64_t parts = free < most ? free : most;
+  p.parts = parts < 1 || p.form == kLarge ? 1u : parts < kMostPerToken ? static_cast<uint32_t>(parts) : kMostPerToken;
   return p;
 }
 
@@ -905,7 +907,9 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
   const uint32_t n_left = out_major ? d.out : d.width, n_right = out_major ? d.width : d.out;
   const void *const left = buffers[out_major ? 1 : 0], *const right = buffers[out_major ? 0 : 1];
-  const GradientPlan plan = gradient_plan(sizeof(T), d.rows, d.experts, d.width, d.out);
+  GradientPlan plan = gradient_plan(sizeof(T), d.rows, d.experts, d.width, d.out);
+  plan.parts = d.per_token < 1 ? 1u : d.per_token;
+  if (plan.parts != 1 && plan.form == kLarge) plan.form = kMiddle;
   const bool direct = whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right);
   const auto run = [&](auto *out) {
     typedef std::remove_pointer_t<decltype(out)> O;
@@ -927,11 +931,10 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
 
 extern "C" {
 
-size_t bpl_expert_matmul_gradient_scratch_bytes(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
-                                                uint32_t element_bytes) {
-  if (experts == 0 || width == 0 || out_width == 0) return 0;
-  const GradientPlan plan = gradient_plan(element_bytes, rows, experts, width, out_width);
-  return plan.parts == 1 ? 0 : static_cast<size_t>(plan.parts) * experts * width * out_width * sizeof(float);
+uint32_t bpl_expert_matmul_gradient_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
+                                          uint32_t element_bytes) {
+  if (experts == 0 || width == 0 || out_width == 0) return 1;
+  return gradient_plan(element_bytes, rows, experts, width, out_width).parts;
 }
 
 BPL_EXPERT_DEFINE(expert_matmul, matmul)

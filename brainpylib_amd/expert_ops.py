@@ -350,10 +350,10 @@ class _ExpertMatmul(torch.autograd.Function):
       d_rows = _matmul(ct, stored, indptr, not ctx.out_major)
     if ctx.needs_input_grad[1]:
       d_stored = torch.empty_like(stored)
-      opaque = _lib.build_expert_descriptor(0, 0, stored.shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
+      parts = _lib.expert_matmul_gradient_parts(rows.shape[0], stored.shape[0], rows.shape[1], ct.shape[1], rows.element_size())
+      scratch = d_stored if parts == 1 else torch.empty((parts,) + tuple(stored.shape), dtype=torch.float32, device=rows.device)
+      opaque = _lib.build_expert_descriptor(0, parts, stored.shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
                                             _OUT_MAJOR if ctx.out_major else 0)
-      scratch = torch.empty(_lib.expert_matmul_gradient_scratch_bytes(rows.shape[0], stored.shape[0], rows.shape[1], ct.shape[1],
-                                                                      rows.element_size()), dtype=torch.uint8, device=rows.device)
       _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct, indptr, d_stored, scratch], opaque)
     sources = (given, rows, stored)
     return _first_order('expert_matmul', d_rows, *sources), _first_order('expert_matmul', d_stored, *sources), None, None

@@ -142,7 +142,7 @@ typedef struct {
  * family; a target reads the fields that its comment names, the others are 0. */
 typedef struct {
   uint32_t tokens;    /* T */
-  uint32_t per_token; /* k: pairs (token, expert) of one token; pair p = t * k + i */
+  uint32_t per_token; /* k: pairs (token, expert) of one token; pair p = t * k + i.  At most 64 */
   uint32_t experts;   /* E, at most 1,024 */
   uint32_t rows;      /* R: rows of the products' left operand */
   uint32_t width;     /* elements of a token's row; the products' inner dimension K */
@@ -162,11 +162,12 @@ typedef struct {
  * doubles, so the kernels see the same log_p as the reference's CPU path. */
 size_t bpl_build_expert_descriptor(uint32_t tokens, uint32_t per_token, uint32_t experts, uint32_t rows, uint32_t width,
                                    uint32_t out_width, uint32_t flags, char *out, size_t cap);
-/* Bytes of scratch memory that expert_sort of so many pairs takes as its last buffer. */
+/* Bytes of scratch memory (at a multiple of 16) that expert_sort of so many pairs takes as its last buffer. */
 size_t bpl_expert_sort_scratch_bytes(uint32_t pairs, uint32_t experts);
-/* The same for expert_matmul_gradient_T; element_bytes: of T. */
-size_t bpl_expert_matmul_gradient_scratch_bytes(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
-                                                uint32_t element_bytes);
+/* Into how many parts (1 to 64) expert_matmul_gradient_T had best split an expert's rows on the current device: results of
+ * few elements over many rows.  element_bytes: of T. */
+uint32_t bpl_expert_matmul_gradient_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
+                                          uint32_t element_bytes);
 size_t bpl_build_event_csr_batching_descriptor(uint32_t n_row, uint32_t n_col, uint32_t batch_size,
                                                uint32_t values_batch, uint32_t indices_batch,
                                                uint32_t indptr_batch, uint32_t events_batch, uint32_t nnz,
@@ -618,8 +619,10 @@ BPL_TARGET(nonzero_double);
  *                          indptr int32[experts + 1], out T[rows][out]]
  *                          out[r] = rows[r] @ weight[e] for indptr[e] <= r < indptr[e + 1] (indptr[0] is taken as 0), zero
  *                          from indptr[experts] on; sums in float
- * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight, scratch]: rows_e^T @ d_out_e, zero for an expert
- *                          without rows.  (The gradient of the rows is expert_matmul with the weight's other storage.)
+ * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight, parts float[per_token][experts][...] as d_weight]:
+ *                          rows_e^T @ d_out_e, zero for an expert without rows.  per_token: the number of parts that an expert's
+ *                          rows are split into (0 or 1: none, and the last buffer is not used).
+ *                          (The gradient of the rows is expert_matmul with the weight's other storage.)
  * ---------------------------------------------------------------------------------------- */
 BPL_TARGET(expert_topk_float);
 BPL_TARGET(expert_topk_half);

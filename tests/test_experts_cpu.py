@@ -43,14 +43,13 @@ def test_sort_scratch_is_for_long_lists_only():
   assert _lib.expert_sort_scratch_bytes(2 ** 31 - 1, 1024) < 1 << 26
 
 
-def test_gradient_scratch_is_the_parts_of_few_results():
-  size = _lib.expert_matmul_gradient_scratch_bytes
-  assert size(100, 8, 2048, 2048, 2) == 0 and size(0, 8, 64, 64, 4) == 0 and size(100_000, 4, 0, 64, 4) == 0
-  assert size(1 << 20, 64, 4096, 4096, 2) == 0
+def test_gradient_is_split_where_results_are_few():
+  parts = _lib.expert_matmul_gradient_parts
+  assert parts(100, 8, 2048, 2048, 2) == 1 and parts(0, 8, 64, 64, 4) == 1 and parts(100_000, 4, 0, 64, 4) == 1
+  assert parts(1 << 20, 64, 4096, 4096, 2) == 1
   for width, out in ((64, 64), (30, 700), (700, 30), (1, 5), (5, 1)):
     for element in (2, 4):
-      n = size(100_000, 2, width, out, element)
-      assert n > 0 and n % (2 * width * out * 4) == 0 and n <= 2 * width * out * 4 * 97
+      assert 1 < parts(100_000, 2, width, out, element) <= 64
 
 
 @pytest.mark.parametrize("call, error", [

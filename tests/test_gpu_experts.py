@@ -356,6 +356,26 @@ def test_matmul_one_at_the_edges_of_the_tiles(cuda, dtype):
         assert torch.equal(got.double().cpu(), want), (n, inner, out)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_matmul_of_the_smallest_and_largest_numbers(cuda, dtype):
+  # numbers below the type's normal ones count, and results beyond its largest are infinite
+  info = torch.finfo(dtype)
+  tiny = info.smallest_normal * info.eps if dtype != torch.float32 else info.smallest_normal / 4
+  rows = torch.zeros(40, 64, dtype=dtype)
+  rows[:, 0], rows[:, 1], rows[:, 2] = 3 * tiny, info.max, info.max
+  weight = torch.zeros(1, 64, 72, dtype=dtype)
+  weight[0, 0, :8] = 1.0 if dtype != torch.float16 else 1024.0
+  weight[0, 1, 8:16], weight[0, 1, 16:24], weight[0, 2, 16:24] = 1.0, 1.0, 1.0
+  weight[0, 1, 24:32], weight[0, 2, 24:32] = 1.0, -1.0
+  indptr = torch.tensor([0, 40], dtype=torch.int32)
+  want = plain.matmul(rows, weight, indptr)
+  for w in (weight.cuda(), weight.transpose(1, 2).contiguous().cuda().transpose(1, 2)):
+    got = bpl.expert_matmul(rows.cuda(), w, indptr.cuda()).cpu()
+    assert torch.equal(got[:, :8].double(), want[:, :8]) and (got[:, :8] != 0).all()
+    assert torch.equal(got[:, 8:16].double(), want[:, 8:16])
+    assert torch.isinf(got[:, 16:24]).all() and (got[:, 24:] == 0).all()
+
+
 def test_matmul_gradients_against_differences(cuda):
   # The product is linear in either operand, so differences of any step are exact but for rounding: 2 products of inner
   # terms, off by check_sums' bound each.
