@@ -207,8 +207,10 @@ __device__ __forceinline__ typename Unit<T, SIDE>::frag fragment(const T *lds, u
 
 // Shape of a tile: BM x BN results, WM x WN waves, matrix instructions of SIDE x SIDE; kStages: of the ring of loads that go straight to LDS, 0: staged through
 // registers into two buffers.
-template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t SIDE, uint32_t STAGES>
+template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t SIDE, uint32_t STAGES, uint32_t LOAD_BYTES = 16>
 struct Shape {
+  static constexpr uint32_t kLoadBytes = LOAD_BYTES;
+  static constexpr uint32_t kWavesWanted = BM_ * BN_ >= 256 * 256 ? 1u : 2u;  // to a SIMD, at least
   static constexpr uint32_t kSide = SIDE, kSteps = kDepthBytes / 16 / (kWave / SIDE);
   static constexpr uint32_t kStages = STAGES;
   // (a wave's room for its results: SIDE rows of 64 columns in 16 bits; of 32 where workgroups are to share a CU)
@@ -349,8 +351,16 @@ constexpr uint32_t kStageDepth = 8;  // pieces of 16 bytes
 template <typename T>
 constexpr uint32_t kStageK = kStageDepth * Piece<T>::kElems;
 
+// BYTES (16, or 4 where lines begin at any element of 32 bits) a lane, side by side in LDS.  ONCE: read once, and to take no room
+// in the caches from what is not.
+template <uint32_t BYTES, bool ONCE>
 __device__ __forceinline__ void load_to_lds(uint32_t lds_bytes, uint32_t offset, const void *base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
+  if constexpr (BYTES == 4)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
+  else if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_bytes), "v"(offset), "s"(base) : "memory");
 }
 template <uint32_t UNDER_WAY>
 __device__ __forceinline__ void wait_for_loads() {
@@ -358,31 +368,33 @@ __device__ __forceinline__ void wait_for_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(UNDER_WAY) : "memory");
 }
 
-template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS>
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS, uint32_t BYTES, bool ONCE>
 struct DirectLoader {
-  static constexpr uint32_t kElems = Piece<T>::kElems;
-  static constexpr uint32_t kPieces = WIDTH * kStageDepth / THREADS;
+  static constexpr uint32_t kElems = Piece<T>::kElems, kParts = 16 / BYTES;  // loads to a piece
+  static constexpr uint32_t kPieces = WIDTH * kStageDepth / THREADS, kLoads = kPieces * kParts;
   static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : kStageDepth;
   static_assert(WIDTH * kStageDepth % THREADS == 0, "whole rounds");
-  uint32_t offset[kPieces];  // bytes from the operand's element (k0, first row)
+  static_assert(BYTES == 16 || BYTES == sizeof(T), "whole elements");
+  uint32_t offset[kLoads];  // bytes from the operand's element (k0, first row)
 
-  // Lane by lane the pieces of LDS are filled in order; place() is its own inverse, so what belongs at place p of a row is
-  // the row's piece place(p).
+  // Lane by lane LDS is filled in order; place() is its own inverse, so what belongs at place p of a row is the row's piece
+  // place(p).
   __device__ __forceinline__ void begin(uint32_t rows, uint32_t stride) {
 #pragma unroll
-    for (uint32_t i = 0; i < kPieces; ++i) {
-      const uint32_t at = threadIdx.x + i * THREADS, line = at / kRowPieces;
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const uint32_t at = (threadIdx.x + i * THREADS) / kParts, within = (threadIdx.x + i * THREADS) % kParts;
+      const uint32_t line = at / kRowPieces;
       const uint32_t piece = place<T, ACROSS, WIDTH, kStageDepth>(line, at % kRowPieces) - line * kRowPieces;
-      if (ACROSS) {  // (columns beyond the last whole piece are not stored: any will do)
-        const uint32_t last = (rows - 1) / kElems;
-        offset[i] = (line * stride + (piece < last ? piece : last) * kElems) * static_cast<uint32_t>(sizeof(T));
+      if (ACROSS) {  // (what is beyond the columns is not stored: any will do)
+        const uint32_t unit = kElems / kParts, last = (rows - 1) / unit, col = piece * kParts + within;
+        offset[i] = (line * stride + (col < last ? col : last) * unit) * static_cast<uint32_t>(sizeof(T));
       } else {
-        offset[i] = ((line < rows ? line : rows - 1) * stride + piece * kElems) * static_cast<uint32_t>(sizeof(T));
+        offset[i] = ((line < rows ? line : rows - 1) * stride + piece * kElems) * static_cast<uint32_t>(sizeof(T)) + within * BYTES;
       }
     }
   }
   __device__ __forceinline__ void load(uint32_t i, const T *base, uint32_t lds_bytes, uint32_t wave) const {
-    load_to_lds(lds_bytes + (i * THREADS + wave * kWave) * 16u, offset[i], base);
+    load_to_lds<BYTES, ONCE>(lds_bytes + (i * THREADS + wave * kWave) * BYTES, offset[i], base);
   }
   // The last stage, of which only `depth` of k are there: by way of registers, with zeros behind.
   static __device__ __forceinline__ void load_partial(const T *__restrict__ base, uint32_t rows, size_t stride, uint32_t depth, T *lds) {
@@ -409,7 +421,8 @@ struct Job {
 };
 
 // jobs(at, &j): the workgroup's next tile from its place `at` on, which begins at 0; false: there are no more.
-template <typename T, typename O, bool A_ACROSS, bool B_ACROSS, typename S, typename JOBS>
+// ONCE: b is read by one tile.
+template <typename T, typename O, bool A_ACROSS, bool B_ACROSS, typename S, bool ONCE, typename JOBS>
 __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_stride, uint32_t b_stride, size_t out_stride,
                                                 float4 *lds, bool past) {
   constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = S::kSteps, kSide = S::kSide, kRing = S::kStages;
@@ -419,9 +432,9 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   const uint32_t wave = uniform(threadIdx.x / kWave);
   const uint32_t m0 = wave / S::WN * (S::BM / S::WM), n0 = wave % S::WN * (S::BN / S::WN);
   const uint32_t lds_base = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) float4 *)lds)));
-  typedef DirectLoader<T, A_ACROSS, S::BM, S::kThreads> LoaderA;
-  typedef DirectLoader<T, B_ACROSS, S::BN, S::kThreads> LoaderB;
-  constexpr uint32_t kLoads = LoaderA::kPieces + LoaderB::kPieces;
+  typedef DirectLoader<T, A_ACROSS, S::BM, S::kThreads, S::kLoadBytes, false> LoaderA;
+  typedef DirectLoader<T, B_ACROSS, S::BN, S::kThreads, S::kLoadBytes, ONCE> LoaderB;
+  constexpr uint32_t kLoads = LoaderA::kLoads + LoaderB::kLoads;
   const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kStageK<T>;
   const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
 
@@ -439,10 +452,10 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   if (more) begin();
   const auto load_one = [&](uint32_t i) {
     const uint32_t to = lds_base + (filled & (kRing - 1)) * kStageBytes;
-    if (i < LoaderA::kPieces)
+    if (i < LoaderA::kLoads)
       load_a.load(i, from.a, to, wave);
     else
-      load_b.load(i - LoaderA::kPieces, from.b, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
+      load_b.load(i - LoaderA::kLoads, from.b, to + kA * static_cast<uint32_t>(sizeof(T)), wave);
   };
   const auto filled_one = [&] {
     from.a += a_step;
@@ -596,7 +609,7 @@ __device__ __forceinline__ void zero_from(T *__restrict__ out, uint32_t first, u
 // as many as fill the card a whole number of times, if those left over fill it at most half; a second launch with a smaller S
 // then takes the smaller tiles of what is left over, on all of the card.
 template <typename T, bool OUT_MAJOR, typename S, typename COARSE>
-__global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
+__global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
                                                               const uint32_t *__restrict__ indptr, T *__restrict__ out,
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
                                                               uint32_t cols, uint32_t split, bool past) {
@@ -634,8 +647,11 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
       return true;
     }
   };
+  // (shapes of few rows are taken where an expert has few: its weights are read once.  403 MB of weights of 64 experts, 8 rows
+  // each: 76 -> 67 us out-major, 84 -> 75 us)
+  constexpr bool kOnce = S::kLoadBytes == 16 && (S::BM == 16 || (S::BM == 64 && sizeof(T) == 2));
   if constexpr (S::kStages != 0) {
-    stream_products<T, T, false, !OUT_MAJOR, S>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds, past);
+    stream_products<T, T, false, !OUT_MAJOR, S, kOnce>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds, past);
   } else {
     Job<T, T> j;
     for (uint32_t at = 0; jobs(at, &j);) {
@@ -652,7 +668,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(const T *__restric
 // stored out-major.  Where there are few tiles an expert's rows are split into `parts`: O = float, part after part, and
 // join_kernel adds them in their order.
 template <typename T, typename O, typename S>
-__global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
+__global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void gradient_kernel(const T *__restrict__ left, const T *__restrict__ right,
                                                                const uint32_t *__restrict__ indptr, O *__restrict__ d_weight,
                                                                uint32_t n_rows, uint32_t experts, uint32_t n_left,
                                                                uint32_t n_right, uint32_t parts, bool past) {
@@ -697,7 +713,7 @@ __global__ __launch_bounds__(S::kThreads) void gradient_kernel(const T *__restri
     return true;
   };
   if constexpr (S::kStages != 0) {
-    stream_products<T, O, true, true, S>(jobs, n_left, n_right, n_right, lds, past);
+    stream_products<T, O, true, true, S, false>(jobs, n_left, n_right, n_right, lds, past);
   } else {
     Job<T, O> j;
     for (uint32_t at = 0; jobs(at, &j);) {
@@ -734,10 +750,10 @@ bool allow_lds(const char *target, K kernel, uint32_t bytes) {
   return false;
 }
 
-// Loads that go straight to LDS need lines at multiples of 16 bytes, and offsets within a tile in 32 bits.
+// Loads of so many bytes that go straight to LDS need lines at multiples of them, and offsets within a tile in 32 bits.
 template <typename T>
-bool whole_pieces(const void *p, uint32_t stride) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % Piece<T>::kElems == 0 && stride < (1u << 20);
+bool straight(const void *p, uint32_t stride, uint32_t bytes = 16) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * sizeof(T) % bytes == 0 && stride < (1u << 20);
 }
 
 // Results of 64 MB and more in whole lines are stored past the caches (32,768 rows, 8 experts of 2,048 x 2,048, bfloat16: 262 ->
@@ -753,6 +769,12 @@ struct Direct {
   using Middle = Shape<128, 128, 2, 2, 32, 2>;
   using Small = Shape<64, 64, 2, 2, 32, 4>;
   using Thin = Shape<16, 64, 1, 2, 16, 4>;
+};
+// (in 32 bits, lines that begin at any element: four loads for one)
+struct DirectWords {
+  using Middle = Shape<128, 128, 2, 2, 32, 2, 4>;
+  using Small = Shape<64, 64, 2, 2, 32, 4, 4>;
+  using Thin = Shape<16, 64, 1, 2, 16, 4, 4>;
 };
 struct Staged {
   using Large = Shape<256, 256, 2, 4, 32, 0>;
@@ -784,18 +806,19 @@ bool launch_product(const char *target, hipStream_t stream, const bpl_expert_des
   return d.flags & BPL_EXPERT_OUT_MAJOR ? launch(product_kernel<T, true, S, COARSE>) : launch(product_kernel<T, false, S, COARSE>);
 }
 
-// Which shape: the least time by the tiles that a CU works through one after the other (those that share it, at least) and a
-// tile's time, measured with the card full of them (32,768 rows, 64 experts, inner dimension 2,048, bfloat16: 60, 19 and 8.5 us;
-// in 32 bits, inner dimension 1,024: 61, 17 and 6 us for the middle, the small and the thin one).  Mean rows of an expert
-// and times of the shapes at 1,536 columns, bfloat16, large / middle / small: 512 rows 239 / 260 / 432, 128 rows 131 / 118 /
-// 147, 16 rows 119 / 86 / 78 us; float32, 1,024 columns, middle / small / thin: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
+// Which shape: the least time by the turns in which the card, full of them, works through a shape's tiles, and a turn's time,
+// measured at many turns (32,768 rows, 64 experts, inner dimension 2,048, bfloat16: 60, 38 and 17 us; in 32 bits, inner
+// dimension 1,024: 122, 34 and 18 us for the middle, the small and the thin one).  The large one is charged a tenth more, which
+// is what tiles that are not full cost it beside the others.  Mean rows of an expert and times of the shapes at 1,536 columns,
+// bfloat16, large / middle / small: 512 rows 239 / 260 / 432, 128 rows 131 / 118 / 147, 16 rows 119 / 86 / 78 us; float32,
+// 1,024 columns, middle / small / thin: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
 enum Form { kLarge, kMiddle, kSmall, kThin };
 struct FormTime {
   Form form;
   uint32_t height, width, share;  // share: workgroups that share a CU
   float time;
 };
-constexpr FormTime kForms16[] = {{kLarge, 256, 256, 1, 60.f}, {kMiddle, 128, 128, 2, 19.f}, {kSmall, 64, 64, 2, 8.5f}};
+constexpr FormTime kForms16[] = {{kLarge, 256, 256, 1, 66.f}, {kMiddle, 128, 128, 2, 19.f}, {kSmall, 64, 64, 2, 8.5f}};
 constexpr FormTime kForms32[] = {{kMiddle, 128, 128, 2, 61.f}, {kSmall, 64, 64, 2, 17.f}, {kThin, 16, 64, 3, 6.f}};
 template <typename TILES>
 Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
@@ -806,7 +829,7 @@ Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
   for (int i = 0; i < 3; ++i) {
     const uint64_t n = tiles(forms[i].height, forms[i].width), held = cus * forms[i].share;
     float turns = static_cast<float>((n + held - 1) / held * forms[i].share);
-    if (split && forms[i].form == kLarge && n % held != 0 && n % held <= held / 2) turns -= 0.35f;
+    if (split && forms[i].form == kLarge && n % held != 0 && n % held <= held / 4) turns -= 0.35f;
     const float time = forms[i].time * turns;
     if (i == 0 || time < least) best = i, least = time;
   }
@@ -816,15 +839,15 @@ Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
 template <typename T, typename SHAPES>
 void choose_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
   // (an expert's last tile is half full on average, and every expert that has rows has one)
-  const Form form = best_form(sizeof(T), d.width >= 512, [&](uint32_t height, uint32_t width) {
+  const bool split = d.width >= 512 && d.rows / d.experts >= 512;
+  const Form form = best_form(sizeof(T), split, [&](uint32_t height, uint32_t width) {
     const uint64_t full = d.rows / height + d.experts / 2, least = d.experts < d.rows ? d.experts : d.rows;
     return (full > least ? full : least) * div_up(d.out, width);
   });
   if constexpr (sizeof(T) == 2) {
     if (form == kLarge) {
-      // A tile that is left over takes a whole turn of the card, 60 us at an inner dimension of 2,048, in quarters 20 to
-      // 40; below 512 of it the second launch costs what that saves.
-      const bool split = d.width >= 512;
+      // (A tile that is left over takes a whole turn of the card, 60 us at an inner dimension of 2,048, in quarters 20 to 40;
+      // below 512 of it the second launch costs what that saves, and of experts of fewer rows the quarters are half empty.)
       if (launch_product<T, typename SHAPES::Large>(target, stream, d, buffers, split) && split)
         launch_product<T, typename SHAPES::Middle, typename SHAPES::Large>(target, stream, d, buffers, true);
       return;
@@ -847,10 +870,13 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
   if (!unpack(target, opaque, opaque_len, &d) || !expert_limits(target, d)) return;
   if (d.rows == 0 || d.out == 0) return;
   const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
-  if (whole_pieces<T>(buffers[0], d.width) && whole_pieces<T>(buffers[1], out_major ? d.width : d.out))
-    choose_product<T, Direct>(target, stream, d, buffers);
-  else
-    choose_product<T, Staged>(target, stream, d, buffers);
+  const uint32_t stride = out_major ? d.width : d.out;
+  if (straight<T>(buffers[0], d.width) && straight<T>(buffers[1], stride)) return choose_product<T, Direct>(target, stream, d, buffers);
+  if constexpr (sizeof(T) == 4) {
+    if (straight<T>(buffers[0], d.width, 4) && straight<T>(buffers[1], stride, 4))
+      return choose_product<T, DirectWords>(target, stream, d, buffers);
+  }
+  choose_product<T, Staged>(target, stream, d, buffers);
 }
 
 // The gradient's shape, and into how many parts an expert's rows are split where the tiles leave places on the card free: at
@@ -910,11 +936,15 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   GradientPlan plan = gradient_plan(sizeof(T), d.rows, d.experts, d.width, d.out);
   plan.parts = d.per_token < 1 ? 1u : d.per_token;
   if (plan.parts != 1 && plan.form == kLarge) plan.form = kMiddle;
-  const bool direct = whole_pieces<T>(left, n_left) && whole_pieces<T>(right, n_right);
   const auto run = [&](auto *out) {
     typedef std::remove_pointer_t<decltype(out)> O;
-    return direct ? choose_gradient<T, O, Direct>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan)
-                  : choose_gradient<T, O, Staged>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
+    if (straight<T>(left, n_left) && straight<T>(right, n_right))
+      return choose_gradient<T, O, Direct>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
+    if constexpr (sizeof(T) == 4) {
+      if (straight<T>(left, n_left, 4) && straight<T>(right, n_right, 4))
+        return choose_gradient<T, O, DirectWords>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
+    }
+    return choose_gradient<T, O, Staged>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
   };
   if (plan.parts == 1) {
     run(static_cast<T *>(buffers[3]));
