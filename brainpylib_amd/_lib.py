@@ -53,7 +53,7 @@ def lib():
                  "bpl_build_matmat_jit_prob_descriptor1", "bpl_build_expert_descriptor",
                  "bpl_expert_sort_scratch_bytes"):
       getattr(l, name).restype = ctypes.c_size_t
-    l.bpl_expert_matmul_gradient_parts.restype = ctypes.c_uint32
+    l.bpl_expert_matmul_parts.restype = l.bpl_expert_matmul_gradient_parts.restype = ctypes.c_uint32
     _lib = l
   return _lib
 
@@ -240,6 +240,14 @@ def expert_sort_scratch_bytes(pairs, experts):
   return lib().bpl_expert_sort_scratch_bytes(ctypes.c_uint32(pairs), ctypes.c_uint32(experts))
 
 
+# (advice: a call goes by the number that it is given, so that one kept from another device is not wrong)
+@functools.lru_cache(maxsize=256)
+def expert_matmul_parts(rows, experts, width, out_width, element_bytes):
+  u = ctypes.c_uint32
+  return lib().bpl_expert_matmul_parts(u(rows), u(experts), u(width), u(out_width), u(element_bytes))
+
+
+@functools.lru_cache(maxsize=256)
 def expert_matmul_gradient_parts(rows, experts, width, out_width, element_bytes):
   u = ctypes.c_uint32
   return lib().bpl_expert_matmul_gradient_parts(u(rows), u(experts), u(width), u(out_width), u(element_bytes))

@@ -608,11 +608,12 @@ __device__ __forceinline__ void zero_from(T *__restrict__ out, uint32_t first, u
 // Tiles are counted in those of `COARSE`.  S = COARSE takes all of them, or, `split` (in workgroups that the card holds at once),
 // as many as fill the card a whole number of times, if those left over fill it at most half; a second launch with a smaller S
 // then takes the smaller tiles of what is left over, on all of the card.
-template <typename T, bool OUT_MAJOR, typename S, typename COARSE>
+// Where there are few tiles the inner dimension is split into `parts`: O = float, part after part, and join_kernel adds them.
+template <typename T, typename O, bool OUT_MAJOR, typename S, typename COARSE>
 __global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void product_kernel(const T *__restrict__ rows, const T *__restrict__ weight,
-                                                              const uint32_t *__restrict__ indptr, T *__restrict__ out,
+                                                              const uint32_t *__restrict__ indptr, O *__restrict__ out,
                                                               uint32_t n_rows, uint32_t experts, uint32_t inner,
-                                                              uint32_t cols, uint32_t split, bool past) {
+                                                              uint32_t cols, uint32_t split, uint32_t parts, bool past) {
   constexpr bool kRest = !std::is_same<S, COARSE>::value;
   constexpr uint32_t kDown = COARSE::BM / S::BM, kAcross = COARSE::BN / S::BN;
   extern __shared__ float4 lds[];
@@ -622,15 +623,22 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void product_kernel(c
   const uint64_t tiles = static_cast<uint64_t>(total) * across;
   uint32_t rest = split != 0 ? static_cast<uint32_t>(tiles % split) : 0u;
   if (rest > split / 2) rest = 0;
-  const Turn turn = turn_of(kRest ? static_cast<uint64_t>(rest) * (kDown * kAcross) : tiles - rest);
-  const auto jobs = [&](uint32_t &at, Job<T, T> *j) {
+  const Turn turn = turn_of(kRest ? static_cast<uint64_t>(rest) * (kDown * kAcross) : (tiles - rest) * parts);
+  const uint32_t length = parts == 1 ? inner : ((inner + parts - 1) / parts + kDepth<T> - 1) / kDepth<T> * kDepth<T>;
+  const auto jobs = [&](uint32_t &at, Job<T, O> *j) {
     for (;;) {
-      uint32_t index = turn.index + at * turn.step, in = 0;
+      uint32_t index = turn.index + at * turn.step, in = 0, k0 = 0;
       if (index >= turn.end) return false;
       ++at;
       if (kRest) {
         in = index % (kDown * kAcross);
         index = static_cast<uint32_t>(tiles - rest) + index / (kDown * kAcross);
+      }
+      uint32_t part = 0;
+      if (parts != 1) {  // (whole stages to a part; the last ones may have none)
+        part = uniform(index % parts);
+        index /= parts;
+        k0 = length * part < inner ? length * part : inner;
       }
       const uint32_t down = uniform(index / across);
       const uint32_t col0 = (index - down * across) * COARSE::BN + in % kAcross * S::BN;
@@ -638,12 +646,12 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void product_kernel(c
       const uint32_t first = tile.first + in / kAcross * S::BM;
       if (first >= tile.end || col0 >= cols) continue;  // (a quarter beyond the tile's rows or columns)
       const T *const w = weight + static_cast<size_t>(tile.expert) * inner * cols;
-      j->a = uniform(rows + static_cast<size_t>(first) * inner);
-      j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner : w + col0);
-      j->out = out + static_cast<size_t>(first) * cols + col0;
+      j->a = uniform(rows + static_cast<size_t>(first) * inner + k0);
+      j->b = uniform(OUT_MAJOR ? w + static_cast<size_t>(col0) * inner + k0 : w + static_cast<size_t>(k0) * cols + col0);
+      j->out = out + (static_cast<size_t>(part) * n_rows + first) * cols + col0;
       j->rows = tile.end - first < S::BM ? tile.end - first : S::BM;
       j->cols = cols - col0 < S::BN ? cols - col0 : S::BN;
-      j->depth = inner;
+      j->depth = inner - k0 < length ? inner - k0 : length;
       return true;
     }
   };
@@ -651,15 +659,15 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void product_kernel(c
   // each: 76 -> 67 us out-major, 84 -> 75 us)
   constexpr bool kOnce = S::kLoadBytes == 16 && (S::BM == 16 || (S::BM == 64 && sizeof(T) == 2));
   if constexpr (S::kStages != 0) {
-    stream_products<T, T, false, !OUT_MAJOR, S, kOnce>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds, past);
+    stream_products<T, O, false, !OUT_MAJOR, S, kOnce>(jobs, inner, OUT_MAJOR ? inner : cols, cols, lds, past);
   } else {
-    Job<T, T> j;
+    Job<T, O> j;
     for (uint32_t at = 0; jobs(at, &j);) {
-      tile_product<T, false, !OUT_MAJOR, S, T>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, inner, j.out, cols, lds);
+      tile_product<T, false, !OUT_MAJOR, S, O>(j.a, j.rows, inner, j.b, j.cols, OUT_MAJOR ? inner : cols, j.depth, j.out, cols, lds);
       __syncthreads();
     }
   }
-  if (kRest) return;
+  if (kRest || parts != 1) return;
   const uint32_t behind = indptr[experts];
   zero_from(out, behind < n_rows ? behind : n_rows, n_rows, cols, S::kThreads);
 }
@@ -723,12 +731,17 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesWanted) void gradient_kernel(
   }
 }
 
+// indptr: rows of `cols` from indptr[experts] on are zero, and have no parts; nullptr: there are none such.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ parts, T *__restrict__ out, size_t n, uint32_t count) {
+__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ parts, T *__restrict__ out, size_t n, uint32_t count,
+                                                   const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t cols) {
+  const size_t there = indptr != nullptr ? static_cast<size_t>(indptr[experts]) * cols : n;
   for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * 256) {
     float sum = 0.f;
+    if (i < there) {
 #pragma unroll 8
-    for (uint32_t p = 0; p < count; ++p) sum += parts[p * n + i];
+      for (uint32_t p = 0; p < count; ++p) sum += parts[p * n + i];
+    }
     out[i] = static_cast<T>(sum);
   }
 }
@@ -783,11 +796,29 @@ struct Staged {
   using Thin = Shape<16, 64, 1, 2, 16, 0>;
 };
 
-// `split`: whether what is left over of COARSE's tiles, when they have filled the card, is given to S.
-template <typename T, typename S, typename COARSE = S>
-bool launch_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers, bool split = false) {
+template <typename T>
+bool join(const char *target, hipStream_t stream, const void *parts, void *out, size_t n, uint32_t count, const void *indptr,
+          uint32_t experts, uint32_t cols) {
+  hipLaunchKernelGGL(join_kernel<T>, dim3(div_up(n, 256) < 4096 ? div_up(n, 256) : 4096), dim3(256), 0, stream,
+                     static_cast<const float *>(parts), static_cast<T *>(out), n, count, static_cast<const uint32_t *>(indptr),
+                     experts, cols);
+  return check_launch(target);
+}
+
+// A product as it is launched.  split: what is left over of COARSE's tiles, when they have filled the card, is for S.
+template <typename O>
+struct Product {
+  const bpl_expert_descriptor &d;
+  void **buffers;
+  O *out;
+  uint32_t parts;
+  bool split;
+};
+template <typename T, typename S, typename COARSE = S, typename O>
+bool launch_product(const char *target, hipStream_t stream, const Product<O> &p) {
+  const bpl_expert_descriptor &d = p.d;
   constexpr uint32_t kDown = COARSE::BM / S::BM * (COARSE::BN / S::BN);
-  const uint64_t tiles = most_tiles(d.rows, d.experts, COARSE::BM) * div_up(d.out, COARSE::BN) * kDown;
+  const uint64_t tiles = most_tiles(d.rows, d.experts, COARSE::BM) * div_up(d.out, COARSE::BN) * kDown * p.parts;
   if (refuse_tiles(target, tiles, 1ull << 31)) return false;
   // one workgroup to each place that the LDS leaves
   const auto held = [](uint32_t lds_bytes) {
@@ -797,13 +828,13 @@ bool launch_product(const char *target, hipStream_t stream, const bpl_expert_des
   const unsigned grid = static_cast<unsigned>(((tiles < places ? tiles : places) + 7) / 8 * 8);
   const auto launch = [&](auto *kernel) {
     if (!allow_lds(target, kernel, S::kLdsBytes)) return false;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLdsBytes, stream,
-                       static_cast<const T *>(buffers[0]), static_cast<const T *>(buffers[1]),
-                       static_cast<const uint32_t *>(buffers[2]), static_cast<T *>(buffers[3]), d.rows, d.experts, d.width,
-                       d.out, split ? held(COARSE::kLdsBytes) : 0u, past_caches(buffers[3], d.rows, d.out, sizeof(T)));
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::kThreads), S::kLdsBytes, stream, static_cast<const T *>(p.buffers[0]),
+                       static_cast<const T *>(p.buffers[1]), static_cast<const uint32_t *>(p.buffers[2]), p.out, d.rows,
+                       d.experts, d.width, d.out, p.split ? held(COARSE::kLdsBytes) : 0u, p.parts,
+                       past_caches(p.out, d.rows, d.out, sizeof(O)));
     return check_launch(target);
   };
-  return d.flags & BPL_EXPERT_OUT_MAJOR ? launch(product_kernel<T, true, S, COARSE>) : launch(product_kernel<T, false, S, COARSE>);
+  return d.flags & BPL_EXPERT_OUT_MAJOR ? launch(product_kernel<T, O, true, S, COARSE>) : launch(product_kernel<T, O, false, S, COARSE>);
 }
 
 // Which shape: the least time by the turns in which the card, full of them, works through a shape's tiles, and a turn's time,
@@ -836,32 +867,60 @@ Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
   return forms[best].form;
 }
 
-template <typename T, typename SHAPES>
-void choose_product(const char *target, hipStream_t stream, const bpl_expert_descriptor &d, void **buffers) {
-  // (an expert's last tile is half full on average, and every expert that has rows has one)
-  const bool split = d.width >= 512 && d.rows / d.experts >= 512;
-  const Form form = best_form(sizeof(T), split, [&](uint32_t height, uint32_t width) {
-    const uint64_t full = d.rows / height + d.experts / 2, least = d.experts < d.rows ? d.experts : d.rows;
-    return (full > least ? full : least) * div_up(d.out, width);
-  });
-  if constexpr (sizeof(T) == 2) {
+// Whether tiles left over by the large ones are worth a second launch: one takes a whole turn of the card, 60 us at an inner
+// dimension of 2,048, in quarters 20 to 40; below 512 of it the launch costs what that saves, and of experts of fewer rows the
+// quarters are half empty.
+bool worth_quarters(const bpl_expert_descriptor &d) { return d.width >= 512 && d.rows / d.experts >= 512; }
+
+// (an expert's last tile is half full on average, and every expert that has rows has one)
+uint64_t likely_tiles(const bpl_expert_descriptor &d, uint32_t height, uint32_t width) {
+  const uint64_t met = d.experts < d.rows ? d.experts : d.rows, full = d.rows / height + met / 2;
+  return (full > met ? full : met) * div_up(d.out, width);
+}
+
+Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
+  return best_form(element_bytes, worth_quarters(d), [&](uint32_t height, uint32_t width) { return likely_tiles(d, height, width); });
+}
+
+// Into how many parts the inner dimension is split where the tiles leave places on the card free, at least 512 of it to a
+// part: where that spares 4 us and the 4 us of the launch that adds them up.  A workgroup's stages come one after the other,
+// 0.25 us each in 16 bits and 0.35 in 32, and the weights at 5 TB/s.  (One row, 4,096 x 64, bfloat16 19 -> 8 + 4 us; two rows on
+// two experts of 2,048 x 1,024, float32 29 -> 13 + 4, bfloat16 11.3 and left as it is, where it would be 7.7 + 4.)
+uint32_t product_parts(uint32_t element_bytes, const bpl_expert_descriptor &d) {
+  const Form form = product_form(element_bytes, d);
+  if (form != kSmall && form != kThin) return 1;
+  const uint32_t height = form == kSmall ? 64 : 16, share = form == kSmall ? 2 : 3;
+  const uint64_t met = d.experts < d.rows ? d.experts : d.rows;
+  uint64_t parts = static_cast<uint64_t>(share) * device_info().num_cu / likely_tiles(d, height, 64);
+  if (parts > d.width / 512) parts = d.width / 512;
+  if (parts > 16) parts = 16;
+  if (parts < 2) return 1;
+  const float whole = (element_bytes == 2 ? 0.25f : 0.35f) * static_cast<float>(d.width / (kDepthBytes / element_bytes));
+  const float bytes = static_cast<float>(met) * static_cast<float>(d.width) * static_cast<float>(d.out) * static_cast<float>(element_bytes) / 5e6f;
+  // (us, both)
+  const float split = whole / static_cast<float>(parts) > bytes ? whole / static_cast<float>(parts) : bytes;
+  return whole - split < 8.f ? 1u : static_cast<uint32_t>(parts);
+}
+
+template <typename T, typename SHAPES, typename O>
+bool choose_product(const char *target, hipStream_t stream, Product<O> p) {
+  Form form = product_form(sizeof(T), p.d);
+  p.split = false;
+  if (p.parts != 1 && form != kThin) form = kSmall;
+  if constexpr (sizeof(T) == 2 && std::is_same<T, O>::value) {
     if (form == kLarge) {
-      // (A tile that is left over takes a whole turn of the card, 60 us at an inner dimension of 2,048, in quarters 20 to 40;
-      // below 512 of it the second launch costs what that saves, and of experts of fewer rows the quarters are half empty.)
-      if (launch_product<T, typename SHAPES::Large>(target, stream, d, buffers, split) && split)
-        launch_product<T, typename SHAPES::Middle, typename SHAPES::Large>(target, stream, d, buffers, true);
-      return;
-    }
-  } else {
-    if (form == kThin) {
-      launch_product<T, typename SHAPES::Thin>(target, stream, d, buffers);
-      return;
+      p.split = worth_quarters(p.d);
+      return launch_product<T, typename SHAPES::Large>(target, stream, p) &&
+             (!p.split || launch_product<T, typename SHAPES::Middle, typename SHAPES::Large>(target, stream, p));
     }
   }
-  if (form == kMiddle)
-    launch_product<T, typename SHAPES::Middle>(target, stream, d, buffers);
-  else
-    launch_product<T, typename SHAPES::Small>(target, stream, d, buffers);
+  if constexpr (sizeof(T) == 4) {
+    if (form == kThin) return launch_product<T, typename SHAPES::Thin>(target, stream, p);
+  }
+  if constexpr (std::is_same<T, O>::value) {
+    if (form == kMiddle) return launch_product<T, typename SHAPES::Middle>(target, stream, p);
+  }
+  return launch_product<T, typename SHAPES::Small>(target, stream, p);
 }
 
 template <typename T>
@@ -869,14 +928,20 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
   bpl_expert_descriptor d;
   if (!unpack(target, opaque, opaque_len, &d) || !expert_limits(target, d)) return;
   if (d.rows == 0 || d.out == 0) return;
-  const bool out_major = (d.flags & BPL_EXPERT_OUT_MAJOR) != 0;
-  const uint32_t stride = out_major ? d.width : d.out;
-  if (straight<T>(buffers[0], d.width) && straight<T>(buffers[1], stride)) return choose_product<T, Direct>(target, stream, d, buffers);
-  if constexpr (sizeof(T) == 4) {
-    if (straight<T>(buffers[0], d.width, 4) && straight<T>(buffers[1], stride, 4))
-      return choose_product<T, DirectWords>(target, stream, d, buffers);
-  }
-  choose_product<T, Staged>(target, stream, d, buffers);
+  const uint32_t stride = d.flags & BPL_EXPERT_OUT_MAJOR ? d.width : d.out, parts = d.per_token < 1 ? 1u : d.per_token;
+  const auto run = [&](auto *out) {
+    const Product<std::remove_pointer_t<decltype(out)>> p{d, buffers, out, parts, false};
+    if (straight<T>(buffers[0], d.width) && straight<T>(buffers[1], stride)) return choose_product<T, Direct>(target, stream, p);
+    if constexpr (sizeof(T) == 4) {
+      if (straight<T>(buffers[0], d.width, 4) && straight<T>(buffers[1], stride, 4))
+        return choose_product<T, DirectWords>(target, stream, p);
+    }
+    return choose_product<T, Staged>(target, stream, p);
+  };
+  if (parts == 1)
+    run(static_cast<T *>(buffers[3]));
+  else if (run(static_cast<float *>(buffers[4])))
+    join<T>(target, stream, buffers[4], buffers[3], static_cast<size_t>(d.rows) * d.out, parts, buffers[2], d.experts, d.out);
 }
 
 // The gradient's shape, and into how many parts an expert's rows are split where the tiles leave places on the card free: at
@@ -951,16 +1016,17 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
     return;
   }
   if (!run(static_cast<float *>(buffers[4]))) return;
-  const size_t n = static_cast<size_t>(d.experts) * n_left * n_right;
-  hipLaunchKernelGGL(join_kernel<T>, dim3(div_up(n, 256) < 4096 ? div_up(n, 256) : 4096), dim3(256), 0, stream,
-                     static_cast<const float *>(buffers[4]), static_cast<T *>(buffers[3]), n, plan.parts);
-  check_launch(target);
+  join<T>(target, stream, buffers[4], buffers[3], static_cast<size_t>(d.experts) * n_left * n_right, plan.parts, nullptr, 0, 0);
 }
 
 }  // namespace
 
 extern "C" {
 
+uint32_t bpl_expert_matmul_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width, uint32_t element_bytes) {
+  if (rows == 0 || experts == 0 || width == 0 || out_width == 0) return 1;
+  return product_parts(element_bytes, bpl_expert_descriptor{0, 0, experts, rows, width, out_width, 0});
+}
 uint32_t bpl_expert_matmul_gradient_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
                                           uint32_t element_bytes) {
   if (experts == 0 || width == 0 || out_width == 0) return 1;

@@ -321,11 +321,13 @@ def expert_combine(rows, weights, order, position):
 # ---- expert_matmul ----------------------------------------------------------------------------------------------------
 def _matmul(rows, stored, indptr, out_major):
   """rows @ weight by expert; ``stored`` is the weight as it lies in memory, (experts, out, inner) where ``out_major``."""
-  out_width = stored.shape[1] if out_major else stored.shape[2]
-  out = torch.empty((rows.shape[0], out_width), dtype=rows.dtype, device=rows.device)
-  opaque = _lib.build_expert_descriptor(0, 0, stored.shape[0], rows.shape[0], rows.shape[1], out_width,
-                                        _OUT_MAJOR if out_major else 0)
-  _call('expert_matmul' + _TYPE_NAME[rows.dtype], [rows, stored, indptr, out], opaque)
+  n, inner = rows.shape
+  experts, out_width = stored.shape[0], stored.shape[1] if out_major else stored.shape[2]
+  out = torch.empty((n, out_width), dtype=rows.dtype, device=rows.device)
+  parts = _lib.expert_matmul_parts(n, experts, inner, out_width, rows.element_size())
+  scratch = out if parts == 1 else torch.empty((parts, n, out_width), dtype=torch.float32, device=rows.device)
+  opaque = _lib.build_expert_descriptor(0, parts, experts, n, inner, out_width, _OUT_MAJOR if out_major else 0)
+  _call('expert_matmul' + _TYPE_NAME[rows.dtype], [rows, stored, indptr, out, scratch], opaque)
   return out
 
 

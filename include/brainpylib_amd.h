@@ -164,6 +164,9 @@ size_t bpl_build_expert_descriptor(uint32_t tokens, uint32_t per_token, uint32_t
                                    uint32_t out_width, uint32_t flags, char *out, size_t cap);
 /* Bytes of scratch memory (at a multiple of 16) that expert_sort of so many pairs takes as its last buffer. */
 size_t bpl_expert_sort_scratch_bytes(uint32_t pairs, uint32_t experts);
+/* Into how many parts (1 to 64) expert_matmul_T had best split the inner dimension on the current device: few results of a long
+ * one.  element_bytes: of T. */
+uint32_t bpl_expert_matmul_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width, uint32_t element_bytes);
 /* Into how many parts (1 to 64) expert_matmul_gradient_T had best split an expert's rows on the current device: results of
  * few elements over many rows.  element_bytes: of T. */
 uint32_t bpl_expert_matmul_gradient_parts(uint32_t rows, uint32_t experts, uint32_t width, uint32_t out_width,
@@ -616,9 +619,10 @@ BPL_TARGET(nonzero_double);
  *                          out[t] = sum over i of weights[t][i] * rows[position[t][i]], in float
  * expert_combine_gradient_T   buffers = [rows, weights, order, position, d_out, d_rows, d_weights]
  * expert_matmul_T          buffers = [rows T[rows][width], weight T[experts][width][out] (out-major: [experts][out][width]),
- *                          indptr int32[experts + 1], out T[rows][out]]
+ *                          indptr int32[experts + 1], out T[rows][out], parts float[per_token][rows][out]]
  *                          out[r] = rows[r] @ weight[e] for indptr[e] <= r < indptr[e + 1] (indptr[0] is taken as 0), zero
- *                          from indptr[experts] on; sums in float
+ *                          from indptr[experts] on; sums in float.  per_token: the number of parts that the inner dimension is
+ *                          split into (0 or 1: none, and the last buffer is not used).
  * expert_matmul_gradient_T buffers = [rows, d_out, indptr, d_weight as weight, parts float[per_token][experts][...] as d_weight]:
  *                          rows_e^T @ d_out_e, zero for an expert without rows.  per_token: the number of parts that an expert's
  *                          rows are split into (0 or 1: none, and the last buffer is not used).

@@ -52,6 +52,15 @@ def test_gradient_is_split_where_results_are_few():
       assert 1 < parts(100_000, 2, width, out, element) <= 64
 
 
+def test_product_is_split_where_results_are_few_and_the_inner_dimension_is_long():
+  parts = _lib.expert_matmul_parts
+  assert parts(0, 8, 4096, 64, 2) == 1 and parts(2, 8, 0, 64, 2) == 1 and parts(2, 8, 1024, 64, 2) == 1
+  assert parts(4096, 8, 4096, 4096, 2) == 1 and parts(512, 64, 4096, 4096, 4) == 1
+  for rows, experts, width, out in ((2, 8, 4096, 264), (3, 5, 4100, 70), (40, 2, 6001, 33), (1, 1024, 2 ** 20, 1)):
+    for element in (2, 4):
+      assert 1 < parts(rows, experts, width, out, element) <= 16
+
+
 @pytest.mark.parametrize("call, error", [
   (lambda: bpl.expert_topk(torch.zeros(2, 4, dtype=torch.float64), k=1), TypeError),
   (lambda: bpl.expert_topk(torch.zeros(2, 4, dtype=torch.int32), k=1), TypeError),

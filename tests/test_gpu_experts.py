@@ -247,7 +247,7 @@ def test_rows_of_more_elements_than_32_bits_number(cuda):
 # ---- expert_matmul ----------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1, 1), (1, 4, 8, 8), (8, 8, 64, 32), (32, 5, 130, 70), (100, 3, 17, 65), (257, 4, 200, 129), (300, 2, 515, 257),
           (900, 7, 96, 384), (1500, 40, 264, 136), (2048, 2, 256, 512), (64, 1024, 40, 48), (700, 3, 1, 33), (700, 3, 33, 1),
-          (1100, 1, 1030, 300)]
+          (1100, 1, 1030, 300), (2, 8, 4096, 264), (3, 5, 4100, 70), (40, 2, 6001, 33)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
