@@ -781,14 +781,21 @@ struct Direct {
   using Large = Shape<256, 256, 2, 2, 32, 2>;
   using Middle = Shape<128, 128, 2, 2, 32, 2>;
   using Small = Shape<64, 64, 2, 2, 32, 4>;
+};
+// In 32 bits: the matrix unit takes longer than loads do, and a third workgroup on a CU is worth more than two stages.
+struct Direct32 {
+  using Middle = Shape<128, 128, 2, 2, 32, 2>;
+  using Small = Shape<64, 64, 2, 2, 32, 2>;
   using Thin = Shape<16, 64, 1, 2, 16, 4>;
 };
-// (in 32 bits, lines that begin at any element: four loads for one)
+// The same for lines that begin at any element: four loads for one.
 struct DirectWords {
   using Middle = Shape<128, 128, 2, 2, 32, 2, 4>;
-  using Small = Shape<64, 64, 2, 2, 32, 4, 4>;
+  using Small = Shape<64, 64, 2, 2, 32, 2, 4>;
   using Thin = Shape<16, 64, 1, 2, 16, 4, 4>;
 };
+template <typename T>
+using DirectOf = std::conditional_t<sizeof(T) == 4, Direct32, Direct>;
 struct Staged {
   using Large = Shape<256, 256, 2, 4, 32, 0>;
   using Middle = Shape<128, 128, 2, 2, 32, 0>;
@@ -889,7 +896,7 @@ Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
 uint32_t product_parts(uint32_t element_bytes, const bpl_expert_descriptor &d) {
   const Form form = product_form(element_bytes, d);
   if (form != kSmall && form != kThin) return 1;
-  const uint32_t height = form == kSmall ? 64 : 16, share = form == kSmall ? 2 : 3;
+  const uint32_t height = form == kSmall ? 64 : 16, share = form == kSmall && element_bytes == 2 ? 2 : 3;
   const uint64_t met = d.experts < d.rows ? d.experts : d.rows;
   uint64_t parts = static_cast<uint64_t>(share) * device_info().num_cu / likely_tiles(d, height, 64);
   if (parts > d.width / 512) parts = d.width / 512;
@@ -931,7 +938,7 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
   const uint32_t stride = d.flags & BPL_EXPERT_OUT_MAJOR ? d.width : d.out, parts = d.per_token < 1 ? 1u : d.per_token;
   const auto run = [&](auto *out) {
     const Product<std::remove_pointer_t<decltype(out)>> p{d, buffers, out, parts, false};
-    if (straight<T>(buffers[0], d.width) && straight<T>(buffers[1], stride)) return choose_product<T, Direct>(target, stream, p);
+    if (straight<T>(buffers[0], d.width) && straight<T>(buffers[1], stride)) return choose_product<T, DirectOf<T>>(target, stream, p);
     if constexpr (sizeof(T) == 4) {
       if (straight<T>(buffers[0], d.width, 4) && straight<T>(buffers[1], stride, 4))
         return choose_product<T, DirectWords>(target, stream, p);
@@ -1004,7 +1011,7 @@ void matmul_gradient(const char *target, hipStream_t stream, void **buffers, con
   const auto run = [&](auto *out) {
     typedef std::remove_pointer_t<decltype(out)> O;
     if (straight<T>(left, n_left) && straight<T>(right, n_right))
-      return choose_gradient<T, O, Direct>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
+      return choose_gradient<T, O, DirectOf<T>>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
     if constexpr (sizeof(T) == 4) {
       if (straight<T>(left, n_left, 4) && straight<T>(right, n_right, 4))
         return choose_gradient<T, O, DirectWords>(target, stream, d, left, right, n_left, n_right, buffers[2], out, plan);
