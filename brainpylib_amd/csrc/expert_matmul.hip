@@ -99,14 +99,14 @@ uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
 // One product kernel body for the three products.  C[m][n] = sum over k of A[m][k] B[n][k], tiles of BM x BN, kDepth (128 bytes
-// of a row) of k at a time through two buffers in LDS.  An operand lies in memory with its k side by side ("along": rows of
+// of a row) of k at a time through buffers in LDS.  An operand lies in memory with its k side by side ("along": rows of
 // tokens, out-major weights) or with its m or n side by side ("across": the others).
 //   along:  LDS holds [m][k], 128 bytes a row; a lane reads the 16 bytes of k that its matrix instruction takes.
 //   across: LDS holds [k][m]; 16-bit types are transposed by the LDS's transposing read (16 lanes read 4 rows of 16
 //           elements and get a column of 4 each), 32-bit ones are read one by one.
 // 16-byte pieces are placed so that the lanes of a read meet different banks (place()).
 template <typename T, uint32_t SIDE>
-struct Unit;  // the matrix instructions of a type: SIDE x SIDE results, one piece (16 bytes) of k from each of the 64 / SIDE lanes of a row
+struct Unit;  // the matrix instructions of a type: SIDE x SIDE results, a piece (16 bytes) of k from each of a row's 64 / SIDE lanes
 #define BPL_UNIT16(TYPE, SIDE, LENGTH, INSTRUCTION)                                                                        \
   template <>                                                                                                              \
   struct Unit<TYPE, SIDE> {                                                                                                \
@@ -136,11 +136,12 @@ constexpr uint32_t kDepthBytes = 128;
 template <typename T>
 constexpr uint32_t kDepth = kDepthBytes / sizeof(T);
 
-// Where piece `piece` of row `row` lies, in pieces of 16 bytes.  along: rows of DEPTH (4 or 8) pieces.  across: rows of WIDTH elements; the
+// Where piece `piece` of row `row` lies, in pieces of 16 bytes.  along: rows of kDepthPieces.  across: rows of WIDTH elements; the
 // 16-bit transposing read takes two neighbouring pieces of four rows.
-template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH>
+constexpr uint32_t kDepthPieces = kDepthBytes / 16;
+template <typename T, bool ACROSS, uint32_t WIDTH>
 __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
-  if (!ACROSS) return row * DEPTH + (piece ^ ((row / (16 / DEPTH)) & (DEPTH - 1u)));
+  if (!ACROSS) return row * kDepthPieces + (piece ^ ((row >> 1) & (kDepthPieces - 1u)));
   constexpr uint32_t kPieces = WIDTH / Piece<T>::kElems;
   if (sizeof(T) == 4) return row * kPieces + piece;
   constexpr uint32_t kPairs = kPieces / 2;  // pairs of pieces in a row: a power of two
@@ -152,9 +153,9 @@ __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
 template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS>
 struct Loader {
   static constexpr uint32_t kElems = Piece<T>::kElems;
-  static constexpr uint32_t kPieces = WIDTH * kDepthBytes / 16 / THREADS;
-  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : 8u;
-  static_assert(WIDTH * kDepthBytes / 16 % THREADS == 0, "whole rounds");
+  static constexpr uint32_t kPieces = WIDTH * kDepthPieces / THREADS;
+  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : kDepthPieces;
+  static_assert(WIDTH * kDepthPieces % THREADS == 0, "whole rounds");
   typename Piece<T>::type held[kPieces];
 
   // base: element (k = 0, first row) of the operand; `rows` of it are there, `stride` elements from one line to the next
@@ -174,19 +175,19 @@ struct Loader {
 #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
       const uint32_t at = threadIdx.x + i * THREADS;
-      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH, 8>(at / kRowPieces, at % kRowPieces)] =
+      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH>(at / kRowPieces, at % kRowPieces)] =
           __builtin_bit_cast(float4, held[i]);
     }
   }
 };
 
 // What a lane gives the matrix unit: of row `row0` + lane % SIDE, piece (64 / SIDE) * step + lane / SIDE of k.
-template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t DEPTH, uint32_t SIDE>
+template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t SIDE>
 __device__ __forceinline__ typename Unit<T, SIDE>::frag fragment(const T *lds, uint32_t row0, uint32_t step) {
   typedef typename Unit<T, SIDE>::frag frag;
   const uint32_t lane = threadIdx.x % kWave, piece = kWave / SIDE * step + lane / SIDE;
   if constexpr (!ACROSS) {
-    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH, DEPTH>(row0 + lane % SIDE, piece)]);
+    return __builtin_bit_cast(frag, reinterpret_cast<const float4 *>(lds)[place<T, false, WIDTH>(row0 + lane % SIDE, piece)]);
   } else if constexpr (sizeof(T) == 4) {
     frag f;
 #pragma unroll
@@ -198,15 +199,15 @@ __device__ __forceinline__ typename Unit<T, SIDE>::frag fragment(const T *lds, u
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) {
       const uint32_t k = piece * 8 + j * 4 + lane % 16 / 4, col = row0 + lane % SIDE / 16 * 16 + lane % 4 * 4;
-      const T *from = lds + place<T, true, WIDTH, DEPTH>(k, col / 8) * 8 + col % 8;
+      const T *from = lds + place<T, true, WIDTH>(k, col / 8) * 8 + col % 8;
       half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) quad *)from);
     }
     return __builtin_bit_cast(frag, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
 }
 
-// Shape of a tile: BM x BN results, WM x WN waves, matrix instructions of SIDE x SIDE; kStages: of the ring of loads that go straight to LDS, 0: staged through
-// registers into two buffers.
+// Shape of a tile: BM x BN results, WM x WN waves, matrix instructions of SIDE x SIDE; kStages: of the ring of loads that go
+// straight to LDS, 0: staged through registers into two buffers.
 template <uint32_t BM_, uint32_t BN_, uint32_t WM_, uint32_t WN_, uint32_t SIDE, uint32_t STAGES, uint32_t LOAD_BYTES = 16>
 struct Shape {
   static constexpr uint32_t kLoadBytes = LOAD_BYTES;
@@ -315,9 +316,9 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
     for (uint32_t step = 0; step < kSteps; ++step) {
       typename Unit<T, S::kSide>::frag fa[S::kFragsM], fb[S::kFragsN];
 #pragma unroll
-      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM, 8, kSide>(at, m0 + i * kSide, step);
+      for (uint32_t i = 0; i < S::kFragsM; ++i) fa[i] = fragment<T, A_ACROSS, S::BM, kSide>(at, m0 + i * kSide, step);
 #pragma unroll
-      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN, 8, kSide>(at + kA, n0 + j * kSide, step);
+      for (uint32_t j = 0; j < S::kFragsN; ++j) fb[j] = fragment<T, B_ACROSS, S::BN, kSide>(at + kA, n0 + j * kSide, step);
 #pragma unroll
       for (uint32_t i = 0; i < S::kFragsM; ++i)
 #pragma unroll
@@ -345,12 +346,14 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
 // may have no other.  (Stages of 64 bytes with four places leave the loads the same time, but ask the L2 twice as often.)
 // A tile's results go out by way of room of their own while the next tile's stages come in.
 //
+// Why these tiles: a wave of 128 x 128 results reads 64 bytes of LDS a cycle and CU for what the matrix unit does, of the 128
+// that LDS gives (64 x 64: 128, which is why smaller tiles are slower: 1,140 / 850 / 480 TFLOP/s for 256 / 128 / 64 squared, 32,768
+// rows, 8 experts of 2,048 x 2,048, bfloat16, out-major; at an inner dimension of 4,096 1,260, a library's plain product 1,470).  Counters of the large
+// one: the matrix units work 60 to 66 % of the cycles (at 1.7 to 1.8 GHz, which is what the card's power allows), waits for
+// stages and for results that go out 20 %; bank conflicts 5 % of LDS cycles.
+//
 // The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
 // counts its own, and waits that count more loads than it knows are longer, never shorter.
-constexpr uint32_t kStageDepth = 8;  // pieces of 16 bytes
-template <typename T>
-constexpr uint32_t kStageK = kStageDepth * Piece<T>::kElems;
-
 // BYTES (16, or 4 where lines begin at any element of 32 bits) a lane, side by side in LDS.  ONCE: read once, and to take no room
 // in the caches from what is not.
 template <uint32_t BYTES, bool ONCE>
@@ -371,9 +374,9 @@ __device__ __forceinline__ void wait_for_loads() {
 template <typename T, bool ACROSS, uint32_t WIDTH, uint32_t THREADS, uint32_t BYTES, bool ONCE>
 struct DirectLoader {
   static constexpr uint32_t kElems = Piece<T>::kElems, kParts = 16 / BYTES;  // loads to a piece
-  static constexpr uint32_t kPieces = WIDTH * kStageDepth / THREADS, kLoads = kPieces * kParts;
-  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : kStageDepth;
-  static_assert(WIDTH * kStageDepth % THREADS == 0, "whole rounds");
+  static constexpr uint32_t kPieces = WIDTH * kDepthPieces / THREADS, kLoads = kPieces * kParts;
+  static constexpr uint32_t kRowPieces = ACROSS ? WIDTH / kElems : kDepthPieces;
+  static_assert(WIDTH * kDepthPieces % THREADS == 0, "whole rounds");
   static_assert(BYTES == 16 || BYTES == sizeof(T), "whole elements");
   uint32_t offset[kLoads];  // bytes from the operand's element (k0, first row)
 
@@ -384,7 +387,7 @@ struct DirectLoader {
     for (uint32_t i = 0; i < kLoads; ++i) {
       const uint32_t at = (threadIdx.x + i * THREADS) / kParts, within = (threadIdx.x + i * THREADS) % kParts;
       const uint32_t line = at / kRowPieces;
-      const uint32_t piece = place<T, ACROSS, WIDTH, kStageDepth>(line, at % kRowPieces) - line * kRowPieces;
+      const uint32_t piece = place<T, ACROSS, WIDTH>(line, at % kRowPieces) - line * kRowPieces;
       if (ACROSS) {  // (what is beyond the columns is not stored: any will do)
         const uint32_t unit = kElems / kParts, last = (rows - 1) / unit, col = piece * kParts + within;
         offset[i] = (line * stride + (col < last ? col : last) * unit) * static_cast<uint32_t>(sizeof(T));
@@ -407,7 +410,7 @@ struct DirectLoader {
       } else {
         if (line < rows && piece * kElems < depth) v = load_piece<T>(base + line * stride, piece * kElems, depth);
       }
-      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH, kStageDepth>(line, piece)] = __builtin_bit_cast(float4, v);
+      reinterpret_cast<float4 *>(lds)[place<T, ACROSS, WIDTH>(line, piece)] = __builtin_bit_cast(float4, v);
     }
   }
 };
@@ -425,7 +428,7 @@ struct Job {
 template <typename T, typename O, bool A_ACROSS, bool B_ACROSS, typename S, bool ONCE, typename JOBS>
 __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_stride, uint32_t b_stride, size_t out_stride,
                                                 float4 *lds, bool past) {
-  constexpr uint32_t kA = S::BM * kStageK<T>, kB = S::BN * kStageK<T>, kSteps = S::kSteps, kSide = S::kSide, kRing = S::kStages;
+  constexpr uint32_t kA = S::BM * kDepth<T>, kB = S::BN * kDepth<T>, kSteps = S::kSteps, kSide = S::kSide, kRing = S::kStages;
   constexpr uint32_t kStageBytes = (kA + kB) * sizeof(T);
   static_assert((kSteps == 4 || kSteps == 2) && (kRing & (kRing - 1)) == 0 && kRing >= 2, "what work() goes by");
   T *const buffer = reinterpret_cast<T *>(lds);
@@ -435,8 +438,8 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   typedef DirectLoader<T, A_ACROSS, S::BM, S::kThreads, S::kLoadBytes, false> LoaderA;
   typedef DirectLoader<T, B_ACROSS, S::BN, S::kThreads, S::kLoadBytes, ONCE> LoaderB;
   constexpr uint32_t kLoads = LoaderA::kLoads + LoaderB::kLoads;
-  const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kStageK<T>;
-  const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kStageK<T>;
+  const size_t a_step = (A_ACROSS ? static_cast<size_t>(a_stride) : 1u) * kDepth<T>;
+  const size_t b_step = (B_ACROSS ? static_cast<size_t>(b_stride) : 1u) * kDepth<T>;
 
   // what is filled: the tile before `filling`, of which `depth_left` of k is left; `filled` and `done` count the stream's stages
   Job<T, O> from;
@@ -460,7 +463,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   const auto filled_one = [&] {
     from.a += a_step;
     from.b += b_step;
-    depth_left -= kStageK<T> < depth_left ? kStageK<T> : depth_left;
+    depth_left -= kDepth<T> < depth_left ? kDepth<T> : depth_left;
     ++filled;
   };
   const auto next_job = [&] {  // the next tile that has anything to fill
@@ -483,11 +486,11 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
     const T *const at = buffer + (stage & (kRing - 1)) * (kA + kB);
     // (in the order in which the products need them)
     if (i == 0)
-      fb[step][0] = fragment<T, B_ACROSS, S::BN, kStageDepth, kSide>(at + kA, n0, step);
+      fb[step][0] = fragment<T, B_ACROSS, S::BN, kSide>(at + kA, n0, step);
     else if (i <= S::kFragsM)
-      fa[step][i - 1] = fragment<T, A_ACROSS, S::BM, kStageDepth, kSide>(at, m0 + (i - 1) * kSide, step);
+      fa[step][i - 1] = fragment<T, A_ACROSS, S::BM, kSide>(at, m0 + (i - 1) * kSide, step);
     else
-      fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kStageDepth, kSide>(at + kA, n0 + (i - S::kFragsM) * kSide, step);
+      fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kSide>(at + kA, n0 + (i - S::kFragsM) * kSide, step);
   };
   // Stage `done`, whose first fragments are held; FILL: there is a whole one to be filled.  `after`: stores that were issued
   // after the loads of the next stage (the counter counts both, in the order in which they were issued).  Behind the stream's
@@ -542,7 +545,7 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   for (uint32_t g = 0; g < kRing; ++g) {
     next_job();
     if (!more) break;
-    if (depth_left >= kStageK<T>) {
+    if (depth_left >= kDepth<T>) {
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) load_one(i);
       filled_one();
@@ -556,10 +559,10 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
   for (uint32_t i = 0; i < kReads; ++i) read_one(0, 0, i);
   Job<T, O> now;
   for (uint32_t at = 0; jobs(at, &now);) {
-    uint32_t left = (now.depth + kStageK<T> - 1) / kStageK<T>;
+    uint32_t left = (now.depth + kDepth<T> - 1) / kDepth<T>;
     while (left != 0) {
       next_job();
-      uint32_t turns = depth_left / kStageK<T>;  // stages with a whole one to fill
+      uint32_t turns = depth_left / kDepth<T>;  // stages with a whole one to fill
       turns = turns < left ? turns : left;
       left -= turns;
       for (; turns != 0; --turns) work(std::true_type());
@@ -903,7 +906,8 @@ uint32_t product_parts(uint32_t element_bytes, const bpl_expert_descriptor &d) {
   if (parts > 16) parts = 16;
   if (parts < 2) return 1;
   const float whole = (element_bytes == 2 ? 0.25f : 0.35f) * static_cast<float>(d.width / (kDepthBytes / element_bytes));
-  const float bytes = static_cast<float>(met) * static_cast<float>(d.width) * static_cast<float>(d.out) * static_cast<float>(element_bytes) / 5e6f;
+  const float bytes = static_cast<float>(met) * static_cast<float>(d.width) * static_cast<float>(d.out) *
+                      static_cast<float>(element_bytes) / 5e6f;
   // (us, both)
   const float split = whole / static_cast<float>(parts) > bytes ? whole / static_cast<float>(parts) : bytes;
   return whole - split < 8.f ? 1u : static_cast<uint32_t>(parts);
@@ -952,8 +956,8 @@ void matmul(const char *target, hipStream_t stream, void **buffers, const char *
 }
 
 // The gradient's shape, and into how many parts an expert's rows are split where the tiles leave places on the card free: at
-// least 512 rows to a part on average (2 experts of 16,384 rows, 64 x 64 results: @SPLIT@).  How many parts there are is the
-// caller's, who brings the room for them; the shape is chosen here.
+// least 512 rows to a part on average (2 experts of 16,384 rows, 64 x 64 results: 58 us, in 32 parts 7 and 3.4 for their sum).
+// How many parts there are is the caller's, who brings the room for them; the shape is chosen here.
 struct GradientPlan {
   Form form;
   uint32_t parts;
