@@ -1,4 +1,8 @@
 """The expert operators on the GPU against plain implementations in 64 bits."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -586,6 +590,36 @@ def test_captured_training_step_replays(cuda):
     torch.cuda.synchronize()
     for a, b in zip(captured, want):
       assert torch.equal(a, b), i
+
+
+def test_captured_cold(cuda):
+  child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "expert_capture_child.py")
+  r = subprocess.run([sys.executable, "-u", child], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+  assert r.returncode == 0 and "captured cold: ok" in r.stdout, r.stdout[-2000:]
+
+
+def test_two_streams_at_once(cuda):
+  # products whose workgroups fill the card, sorts with room of their own: each as if it were alone
+  indptr = torch.tensor([0, 1500, 1500, 4000], dtype=torch.int32).cuda()
+  operands = [(normal(i, 4000, 512, dtype=torch.bfloat16).cuda(), normal(10 + i, 3, 512, 640, dtype=torch.bfloat16).cuda(),
+               torch.from_numpy(choices(i, 20_000, 4, 40)).cuda()) for i in range(2)]
+
+  def work(x, w, chosen):
+    return (bpl.expert_matmul(x, w, indptr),) + bpl.expert_sort(chosen, num_experts=40)
+
+  want = [work(*o) for o in operands]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream() for _ in operands]
+  got = [[], []]
+  for _ in range(8):
+    for s, o, g in zip(streams, operands, got):
+      with torch.cuda.stream(s):
+        g.append(work(*o))
+  torch.cuda.synchronize()
+  for g, w in zip(got, want):
+    for result in g:
+      for a, b in zip(result, w):
+        assert torch.equal(a, b)
 
 
 def test_captured_sort_of_many_pairs_replays(cuda):
