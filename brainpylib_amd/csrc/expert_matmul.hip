@@ -347,15 +347,16 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
 // A tile's results go out by way of room of their own while the next tile's stages come in.
 //
 // Why these tiles: a wave of 128 x 128 results reads 64 bytes of LDS a cycle and CU for what the matrix unit does, of the 128
-// that LDS gives (64 x 64: 128, which is why smaller tiles are slower: 1,140 / 850 / 480 TFLOP/s for 256 / 128 / 64 squared, 32,768
-// rows, 8 experts of 2,048 x 2,048, bfloat16, out-major; at an inner dimension of 4,096 1,260, a library's plain product 1,470).  Counters of the large
-// one: the matrix units work 60 to 66 % of the cycles (at 1.7 to 1.8 GHz, which is what the card's power allows), waits for
-// stages and for results that go out 20 %; bank conflicts 5 % of LDS cycles.
+// that LDS gives (64 x 64: 128, which is why smaller tiles are slower: 1,140 / 850 / 480 TFLOP/s for 256 / 128 / 64 squared,
+// 32,768 rows, 8 experts of 2,048 x 2,048, bfloat16, out-major; at an inner dimension of 4,096 1,260, a library's plain product
+// 1,470).  Counters of the large one: the matrix units work 60 to 66 % of the cycles (at 1.7 to 1.8 GHz, which is what the
+// card's power allows), waits for stages and for results that go out 20 %; bank conflicts 5 % of LDS cycles.
 //
 // The compiler knows nothing of these loads (its own form waits for every one of them before any read of LDS): it only
 // counts its own, and waits that count more loads than it knows are longer, never shorter.
-// BYTES (16, or 4 where lines begin at any element of 32 bits) a lane, side by side in LDS.  ONCE: read once, and to take no room
-// in the caches from what is not.
+
+// BYTES (16, or 4 where lines begin at any element of 32 bits) a lane, side by side in LDS.  ONCE: read once, and to take no
+// room in the caches from what is not.
 template <uint32_t BYTES, bool ONCE>
 __device__ __forceinline__ void load_to_lds(uint32_t lds_bytes, uint32_t offset, const void *base) {
   if constexpr (BYTES == 4)
@@ -493,8 +494,9 @@ __device__ __forceinline__ void stream_products(const JOBS &jobs, uint32_t a_str
       fb[step][i - S::kFragsM] = fragment<T, B_ACROSS, S::BN, kSide>(at + kA, n0 + (i - S::kFragsM) * kSide, step);
   };
   // Stage `done`, whose first fragments are held; FILL: there is a whole one to be filled.  `after`: stores that were issued
-  // after the loads of the next stage (the counter counts both, in the order in which they were issued).  Behind the stream's
-  // last stage something is read as well, which nothing uses.
+  // after the loads of the next stage (the counter counts both, in the order in which they were issued).  A partial stage is no
+  // load under way; the wait beside its fill is for all of them, so that none older is left where the counts take it for one.
+  // Behind the stream's last stage something is read as well, which nothing uses.
   constexpr uint32_t kStores = S::BM / S::WM * (S::BN / S::WN) / kWave / Piece<O>::kElems;  // of a wave's tile
   bool after = false;
   const auto work = [&](auto FILL) {

@@ -450,9 +450,9 @@ __device__ __forceinline__ float lane_value(float v, uint32_t i) { return __uint
 
 // ---- the rows' two ways ---------------------------------------------------------------------------------------------
 // Bound by memory.  A wave takes a piece of 64 * 16 bytes of a token's row, reads it once and writes it k times (or the other
-// way round): 16,385 tokens of 2,048 bfloat16 to 8 experts each 104 us, 5.8 TB/s.  Its lanes read the token's positions side by side and look
-// up what the rows there say (a pair counts only where order and position answer each other, so that no arrays, however
-// made, lead two tokens to one row or beyond the arrays).
+// way round): 16,385 tokens of 2,048 bfloat16 to 8 experts each 104 us, 5.8 TB/s.  Its lanes read the token's positions side
+// by side and look up what the rows there say (a pair counts only where order and position answer each other, so that no
+// arrays, however made, lead two tokens to one row or beyond the arrays).
 struct Pair {
   uint32_t row;  // kNone: no row
   bool answered;

@@ -205,7 +205,8 @@ def expert_sort(experts, *, num_experts: int):
     return torch.empty(shape, dtype=torch.int32, device=experts.device)
 
   indptr, order, position = ints(num_experts + 1), ints(pairs), ints(*experts.shape)
-  scratch = ints(_lib.expert_sort_scratch_bytes(pairs, num_experts) // 4)
+  room = _lib.expert_sort_scratch_bytes(pairs, num_experts)
+  scratch = ints(room // 4) if room else indptr  # (not used)
   opaque = _lib.build_expert_descriptor(pairs, 1, num_experts, 0, 0, 0, 0)
   _call('expert_sort', [experts, indptr, order, position, scratch], opaque)
   return indptr, order, position
