@@ -261,11 +261,13 @@ void topk_gradient(const char *target, hipStream_t stream, void **buffers, const
 // (workgroup, expert) by one launch (none where one workgroup takes all), then every workgroup adds up the counts before
 // its own, scans the experts and ranks its pairs 64 at a time, in their order.  What is dropped counts as one more
 // expert behind the last.  No atomics but in counts, so the result never depends on an order.
-// Bound by the chain of its steps, not by bytes: 524,296 pairs over 256 experts 14.8 us, of which the two launches 4.8 and 12.
+// Bound by the chain of its steps, not by bytes: 524,296 pairs over 256 experts 14.1 us, in two
+// launches of 4.8 and 11 (14.8 with eight rows of counts and no next steps under way).
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / kWave;
 constexpr uint32_t kSortPairs = 2048;  // to a workgroup, at least
 constexpr uint32_t kSortOne = 8192;    // so many pairs one workgroup takes alone
 constexpr uint32_t kSortMostGroups = 256;
+constexpr uint32_t kSortRows = 20;      // rows of counts that a thread requests together
 constexpr uint32_t kSortAtOnce = 4;    // steps of 64 pairs whose experts a wave requests together
 
 struct SortShape {
@@ -283,23 +285,34 @@ SortShape sort_shape(uint32_t pairs) {
 // A workgroup's row of counts: one for each expert and one for what is dropped, in whole quads.
 __host__ __device__ inline uint32_t sort_bins(uint32_t experts) { return (experts + 4u) / 4u * 4u; }
 
-// f(step, expert, whether there is a pair) for a wave's pairs from `first` on, 64 a step.
+// The experts of a wave's pairs from `first + i0` on, kSortAtOnce steps of 64.
+struct SortSteps {
+  uint32_t e[kSortAtOnce];
+};
+__device__ __forceinline__ SortSteps sort_load(const uint32_t *__restrict__ chosen, uint64_t first, uint32_t i0, uint32_t part,
+                                               uint32_t pairs) {
+  SortSteps s;
+#pragma unroll
+  for (uint32_t j = 0; j < kSortAtOnce; ++j) {
+    const uint32_t i = i0 + j * kWave;
+    const uint64_t p = first + i + threadIdx.x % kWave;
+    s.e[j] = i < part && p < pairs ? chosen[p] : 0u;
+  }
+  return s;
+}
+// f(pair, expert, whether there is a pair) for a wave's pairs from `first` on, 64 a step; `now`: the first steps' experts.  The
+// next ones are requested before these are worked on.
 template <typename FN>
 __device__ __forceinline__ void sort_steps(const uint32_t *__restrict__ chosen, uint64_t first, uint32_t part, uint32_t pairs,
-                                           uint32_t experts, FN f) {
-  const uint32_t lane = threadIdx.x % kWave;
+                                           uint32_t experts, SortSteps now, FN f) {
   for (uint32_t i0 = 0; i0 < part; i0 += kSortAtOnce * kWave) {
-    uint32_t e[kSortAtOnce];
+    const SortSteps next = sort_load(chosen, first, i0 + kSortAtOnce * kWave, part, pairs);
 #pragma unroll
     for (uint32_t j = 0; j < kSortAtOnce; ++j) {
-      const uint64_t p = first + i0 + j * kWave + lane;
-      e[j] = i0 + j * kWave < part && p < pairs ? chosen[p] : 0u;
+      const uint64_t p = first + i0 + j * kWave + threadIdx.x % kWave;
+      if (i0 + j * kWave < part) f(p, now.e[j] < experts ? now.e[j] : experts, p < pairs);
     }
-#pragma unroll
-    for (uint32_t j = 0; j < kSortAtOnce; ++j) {
-      const uint64_t p = first + i0 + j * kWave + lane;
-      if (i0 + j * kWave < part) f(p, e[j] < experts ? e[j] : experts, p < pairs);
-    }
+    now = next;
   }
 }
 
@@ -307,11 +320,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const uint32_t
                                                                   uint32_t pairs, uint32_t experts, uint32_t share) {
   __shared__ uint32_t count[kMostExperts + 4];
   const uint32_t bins = sort_bins(experts);
-  for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) count[e] = 0;
-  __syncthreads();
   const uint32_t part = share / kSortWaves;
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * share + threadIdx.x / kWave * part;
-  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t, uint32_t e, bool there) {
+  const SortSteps ahead = sort_load(chosen, first, 0, part, pairs);
+  for (uint32_t e = threadIdx.x; e < bins; e += kSortThreads) count[e] = 0;
+  __syncthreads();
+  sort_steps(chosen, first, part, pairs, experts, ahead, [&](uint64_t, uint32_t e, bool there) {
     if (there) atomicAdd(&count[e], 1u);
   });
   __syncthreads();
@@ -329,25 +343,31 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
   uint32_t *const total = next + kSortWaves * bins, *const before = total + bins;
   __shared__ uint32_t wave_total[kSortWaves];
   const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  for (uint32_t i = threadIdx.x; i < (kSortWaves + 2) * bins; i += kSortThreads) next[i] = 0;
-  __syncthreads();
   uint32_t *const mine = next + wave * bins;
   const uint32_t part = share / kSortWaves;  // (a multiple of 64)
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * share + wave * part;
+  const SortSteps ahead = sort_load(chosen, first, 0, part, pairs);
+  for (uint32_t i = threadIdx.x; i < (kSortWaves + 2) * bins; i += kSortThreads) next[i] = 0;
+  __syncthreads();
   if (groups != 1) {
     // four experts to a lane, lanes side by side; sets of them share the workgroups' counts
     const uint32_t quads = bins / 4, sets = kSortThreads / quads, set = threadIdx.x / quads, quad = threadIdx.x % quads;
     if (set < sets) {
       uint4 all = make_uint4(0, 0, 0, 0), below = all;
       const uint4 *const from = reinterpret_cast<const uint4 *>(counts) + quad;
-      // (a share to a set, its rows one after the other: eight requests under way)
+      // (a share to a set, kSortRows rows of it requested together: what is beyond is not read one by one)
       const uint32_t rows = (groups + sets - 1) / sets, b0 = set * rows, b1 = b0 + rows < groups ? b0 + rows : groups;
-#pragma unroll 8
-      for (uint32_t b = b0; b < b1; ++b) {
-        const uint4 c = from[static_cast<size_t>(b) * quads];
-        const uint32_t mask = b < blockIdx.x ? 0xffffffffu : 0u;
-        all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
-        below.x += c.x & mask, below.y += c.y & mask, below.z += c.z & mask, below.w += c.w & mask;
+      for (uint32_t b = b0; b < b1; b += kSortRows) {
+        uint4 c[kSortRows];
+#pragma unroll
+        for (uint32_t j = 0; j < kSortRows; ++j)
+          c[j] = b + j < b1 ? from[static_cast<size_t>(b + j) * quads] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t j = 0; j < kSortRows; ++j) {
+          const uint32_t mask = b + j < blockIdx.x ? 0xffffffffu : 0u;
+          all.x += c[j].x, all.y += c[j].y, all.z += c[j].z, all.w += c[j].w;
+          below.x += c[j].x & mask, below.y += c[j].y & mask, below.z += c[j].z & mask, below.w += c[j].w & mask;
+        }
       }
       atomicAdd(&total[4 * quad], all.x), atomicAdd(&total[4 * quad + 1], all.y);
       atomicAdd(&total[4 * quad + 2], all.z), atomicAdd(&total[4 * quad + 3], all.w);
@@ -355,7 +375,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
       atomicAdd(&before[4 * quad + 2], below.z), atomicAdd(&before[4 * quad + 3], below.w);
     }
   }
-  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t, uint32_t e, bool there) {
+  sort_steps(chosen, first, part, pairs, experts, ahead, [&](uint64_t, uint32_t e, bool there) {
     if (there) atomicAdd(&mine[e], 1u);
   });
   __syncthreads();
@@ -404,7 +424,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const uint32_t
   __syncthreads();
   const uint32_t bits = 32u - __builtin_clz(experts);
   volatile uint32_t *const places = mine;
-  sort_steps(chosen, first, part, pairs, experts, [&](uint64_t p, uint32_t e, bool there) {
+  sort_steps(chosen, first, part, pairs, experts, ahead, [&](uint64_t p, uint32_t e, bool there) {
     uint64_t same = __ballot(there);
     for (uint32_t b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((e >> b) & 1u);
