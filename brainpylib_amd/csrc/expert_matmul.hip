@@ -849,31 +849,42 @@ bool launch_product(const char *target, hipStream_t stream, const Product<O> &p)
   return d.flags & BPL_EXPERT_OUT_MAJOR ? launch(product_kernel<T, O, true, S, COARSE>) : launch(product_kernel<T, O, false, S, COARSE>);
 }
 
-// Which shape: the least time by the turns in which the card, full of them, works through a shape's tiles, and a turn's time,
-// measured at many turns (32,768 rows, 64 experts, inner dimension 2,048, bfloat16: 60, 38 and 17 us; in 32 bits, inner
-// dimension 1,024: 122, 34 and 18 us for the middle, the small and the thin one).  The large one is charged a tenth more, which
-// is what tiles that are not full cost it beside the others.  Mean rows of an expert and times of the shapes at 1,536 columns,
-// bfloat16, large / middle / small: 512 rows 239 / 260 / 432, 128 rows 131 / 118 / 147, 16 rows 119 / 86 / 78 us; float32,
-// 1,024 columns, middle / small / thin: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
+// Which shape: the least time by the turns in which the card, full of them, works through a shape's tiles.  A turn's time, in us:
+// `fixed` and, for 2,048 of the inner dimension (in the gradient: of rows to an expert), `deep`; the large shape has one
+// workgroup to a CU, so that nothing goes on there while a tile begins and ends.  `alone`: of a turn that leaves every CU at most
+// one workgroup where two could share it; of a fuller one the share that its tiles have.
+// Fitted to 528 products in 16 bits (32 and 128 experts, inner dimensions of 1,024 to 8,192, 768 to 2,048 columns, both
+// storages, 4 to 800 rows to an expert) and 144 gradients (8 to 128 experts, 16 to 4,096 rows to one), every shape timed at each:
+// the chosen one takes less than 1 % longer than the best on average (5 % and up to 1.67 times, with a time by turns alone), at
+// most 1.28 times, where experts' last tiles fill up a turn or do not.  Times of large / middle / small: 128 experts of 448 rows, 8,192 x 1,536, bfloat16, in-major 1,580 / 2,436; 32 experts of
+// 320 rows, 1,024 x 768 51 / 30; of 16 rows, 2,048 x 1,536 119 / 86 / 78 (64 experts).  In 32 bits by turns alone, at an
+// inner dimension of 1,024; middle / small / thin, 1,024 columns: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
 enum Form { kLarge, kMiddle, kSmall, kThin };
 struct FormTime {
   Form form;
   uint32_t height, width, share;  // share: workgroups that share a CU
-  float time;
+  float fixed, deep, alone;
 };
-constexpr FormTime kForms16[] = {{kLarge, 256, 256, 1, 66.f}, {kMiddle, 128, 128, 2, 19.f}, {kSmall, 64, 64, 2, 8.5f}};
-constexpr FormTime kForms32[] = {{kMiddle, 128, 128, 2, 61.f}, {kSmall, 64, 64, 2, 17.f}, {kThin, 16, 64, 3, 6.f}};
+constexpr FormTime kProduct16[] = {
+    {kLarge, 256, 256, 1, 24.f, 46.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 40.f, 0.6f}, {kSmall, 64, 64, 2, 2.f, 17.f, 0.6f}};
+constexpr FormTime kGradient16[] = {
+    {kLarge, 256, 256, 1, 8.f, 42.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 42.f, 1.f}, {kSmall, 64, 64, 2, 1.f, 17.f, 1.f}};
+constexpr FormTime kEither32[] = {
+    {kMiddle, 128, 128, 2, 0.f, 122.f, 1.f}, {kSmall, 64, 64, 2, 0.f, 34.f, 1.f}, {kThin, 16, 64, 3, 0.f, 18.f, 1.f}};
 template <typename TILES>
-Form best_form(uint32_t element_bytes, bool split, TILES tiles) {
-  const FormTime *const forms = element_bytes == 2 ? kForms16 : kForms32;
+Form best_form(const FormTime (&forms)[3], uint32_t depth, bool split, TILES tiles) {
   const uint64_t cus = device_info().num_cu;
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 3; ++i) {
-    const uint64_t n = tiles(forms[i].height, forms[i].width), held = cus * forms[i].share;
-    float turns = static_cast<float>((n + held - 1) / held * forms[i].share);
-    if (split && forms[i].form == kLarge && n % held != 0 && n % held <= held / 4) turns -= 0.35f;
-    const float time = forms[i].time * turns;
+    const uint64_t n = tiles(forms[i].height, forms[i].width), held = cus * forms[i].share, rest = n % held;
+    float turns = static_cast<float>(n / held);
+    if (rest != 0) {
+      const float full = static_cast<float>(rest) / static_cast<float>(held);
+      turns += full <= 0.5f ? forms[i].alone : forms[i].alone + (1.f - forms[i].alone) * (2.f * full - 1.f);
+    }
+    if (split && forms[i].form == kLarge && rest != 0 && rest <= held / 4) turns -= 0.35f;
+    const float time = (forms[i].fixed + forms[i].deep * static_cast<float>(depth) / 2048.f) * turns;
     if (i == 0 || time < least) best = i, least = time;
   }
   return forms[best].form;
@@ -891,7 +902,8 @@ uint64_t likely_tiles(const bpl_expert_descriptor &d, uint32_t height, uint32_t 
 }
 
 Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
-  return best_form(element_bytes, worth_quarters(d), [&](uint32_t height, uint32_t width) { return likely_tiles(d, height, width); });
+  return best_form(element_bytes == 2 ? kProduct16 : kEither32, d.width, worth_quarters(d),
+                   [&](uint32_t height, uint32_t width) { return likely_tiles(d, height, width); });
 }
 
 // Into how many parts the inner dimension is split where the tiles leave places on the card free, at least 512 of it to a
@@ -969,7 +981,8 @@ GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t exper
     return static_cast<uint64_t>(experts) * div_up(inner, height) * div_up(out, width);
   };
   GradientPlan p;
-  p.form = best_form(element_bytes, false, tiles);
+  const uint32_t mean = rows / experts;  // (a tile of few rows begins and ends as well)
+  p.form = best_form(element_bytes == 2 ? kGradient16 : kEither32, mean < 64 ? 64 : mean, false, tiles);
   if (p.form == kThin) p.form = kSmall;
   const uint32_t side = p.form == kLarge ? 256 : p.form == kMiddle ? 128 : 64;
   const uint64_t free = 2ull * device_info().num_cu / tiles(side, side), most = rows / experts / 512;
