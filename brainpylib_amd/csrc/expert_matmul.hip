@@ -857,8 +857,10 @@ bool launch_product(const char *target, hipStream_t stream, const Product<O> &p)
 // storages, 4 to 800 rows to an expert) and 144 gradients (8 to 128 experts, 16 to 4,096 rows to one), every shape timed at each:
 // the chosen one takes less than 1 % longer than the best on average (5 % and up to 1.67 times, with a time by turns alone), at
 // most 1.28 times, where experts' last tiles fill up a turn or do not.  Times of large / middle / small: 128 experts of 448 rows, 8,192 x 1,536, bfloat16, in-major 1,580 / 2,436; 32 experts of
-// 320 rows, 1,024 x 768 51 / 30; of 16 rows, 2,048 x 1,536 119 / 86 / 78 (64 experts).  In 32 bits by turns alone, at an
-// inner dimension of 1,024; middle / small / thin, 1,024 columns: 512 rows 552 / 586 / 788, 16 rows 128 / 76 / 64.
+// 320 rows, 1,024 x 768 51 / 30; of 16 rows, 2,048 x 1,536 119 / 86 / 78 (64 experts).
+// In 32 bits 356 products (7 to 128 experts, 512 to 4,096 x 512 to 1,536, both storages, odd ones, 2 to 700 rows): half a percent
+// over the best on average, at most 1.2 times (4 % and 1.75 by turns alone); 168 gradients by turns alone, 2 % and 1.14.
+// Middle / small / thin: 128 experts of 32 rows, 2,048 x 1,536 729 / 440 / 677, 7 of 8, 1,024 x 1,024 67 / 23 / 16.
 enum Form { kLarge, kMiddle, kSmall, kThin };
 struct FormTime {
   Form form;
@@ -869,8 +871,10 @@ constexpr FormTime kProduct16[] = {
     {kLarge, 256, 256, 1, 24.f, 46.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 40.f, 0.6f}, {kSmall, 64, 64, 2, 2.f, 17.f, 0.6f}};
 constexpr FormTime kGradient16[] = {
     {kLarge, 256, 256, 1, 8.f, 42.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 42.f, 1.f}, {kSmall, 64, 64, 2, 1.f, 17.f, 1.f}};
-constexpr FormTime kEither32[] = {
-    {kMiddle, 128, 128, 2, 0.f, 122.f, 1.f}, {kSmall, 64, 64, 2, 0.f, 34.f, 1.f}, {kThin, 16, 64, 3, 0.f, 18.f, 1.f}};
+constexpr FormTime kProduct32[] = {
+    {kMiddle, 128, 128, 2, 8.f, 244.f, 0.75f}, {kSmall, 64, 64, 2, 2.f, 68.f, 0.75f}, {kThin, 16, 64, 3, 0.f, 66.f, 0.75f}};
+constexpr FormTime kGradient32[] = {
+    {kMiddle, 128, 128, 2, 0.f, 244.f, 1.f}, {kSmall, 64, 64, 2, 0.f, 68.f, 1.f}, {kThin, 16, 64, 3, 0.f, 68.f, 1.f}};
 template <typename TILES>
 Form best_form(const FormTime (&forms)[3], uint32_t depth, bool split, TILES tiles) {
   const uint64_t cus = device_info().num_cu;
@@ -902,7 +906,7 @@ uint64_t likely_tiles(const bpl_expert_descriptor &d, uint32_t height, uint32_t 
 }
 
 Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
-  return best_form(element_bytes == 2 ? kProduct16 : kEither32, d.width, worth_quarters(d),
+  return best_form(element_bytes == 2 ? kProduct16 : kProduct32, d.width, worth_quarters(d),
                    [&](uint32_t height, uint32_t width) { return likely_tiles(d, height, width); });
 }
 
@@ -982,7 +986,7 @@ GradientPlan gradient_plan(uint32_t element_bytes, uint32_t rows, uint32_t exper
   };
   GradientPlan p;
   const uint32_t mean = rows / experts;  // (a tile of few rows begins and ends as well)
-  p.form = best_form(element_bytes == 2 ? kGradient16 : kEither32, mean < 64 ? 64 : mean, false, tiles);
+  p.form = best_form(element_bytes == 2 ? kGradient16 : kGradient32, mean < 64 ? 64 : mean, false, tiles);
   if (p.form == kThin) p.form = kSmall;
   const uint32_t side = p.form == kLarge ? 256 : p.form == kMiddle ? 128 : 64;
   const uint64_t free = 2ull * device_info().num_cu / tiles(side, side), most = rows / experts / 512;
