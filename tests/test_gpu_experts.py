@@ -300,6 +300,33 @@ def test_matmul_of_many_tiles(cuda, dtype, out_major, n, experts, inner, out):
   check_sums(d_weight, want[1], size[1], int((indptr[1:] - indptr[:-1]).max()) + 1, "d_weight")
 
 
+@pytest.mark.parametrize("dtype, out_major, inner, out", [
+  (torch.bfloat16, True, 4160, 1024), (torch.float16, False, 4160, 1024), (torch.bfloat16, False, 4100, 1000), (torch.float16, True, 4163, 1001)])
+def test_matmul_of_many_large_tiles(cuda, dtype, out_major, inner, out):
+  # a long inner dimension: the largest tiles, those left over in quarters, in whole pieces and not; one expert has no rows.
+  # Whole numbers: every sum is exact in 32 bits in any order (below 2 * 7,800 < 2^24), one rounding is left, and it is to nearest
+  # on both sides.
+  indptr = torch.tensor([0, 5200, 5200, 13_000, 19_900], dtype=torch.int32)
+  n, experts = 20_000, 4
+  g = torch.Generator().manual_seed(inner)
+  rows = torch.randint(-2, 3, (n, inner), generator=g).to(dtype).cuda()
+  ct = torch.randint(-1, 2, (n, out), generator=g).to(dtype).cuda()
+  weight = torch.randint(-1, 2, (experts, inner, out), generator=g).to(dtype).cuda()
+  rows[19_900:], ct[19_900:] = float("nan"), float("nan")
+  given = rows.clone().requires_grad_()
+  stored = (weight.transpose(1, 2).contiguous() if out_major else weight).clone().requires_grad_()
+  got = bpl.expert_matmul(given, stored.transpose(1, 2) if out_major else stored, indptr.cuda())
+  d_rows, d_stored = torch.autograd.grad(got, (given, stored), ct)
+  d_weight = d_stored.transpose(1, 2) if out_major else d_stored
+  for e in range(experts):
+    at = slice(int(indptr[e]), int(indptr[e + 1]))
+    x, c, w = rows[at].float(), ct[at].float(), weight[e].float()
+    assert torch.equal(got[at], (x @ w).to(dtype)), e
+    assert torch.equal(d_rows[at], (c @ w.t().contiguous()).to(dtype)), e
+    assert torch.equal(d_weight[e], (x.t().contiguous() @ c).to(dtype)), e
+  assert (got[19_900:] == 0).all() and (d_rows[19_900:] == 0).all()
+
+
 def test_results_that_are_stored_past_the_caches(cuda):
   # more than 64 MB in whole lines: products, rows to the experts and the gradients
   indptr = torch.tensor([0, 20_000, 20_000, 33_000], dtype=torch.int32)
