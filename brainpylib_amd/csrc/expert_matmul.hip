@@ -869,6 +869,9 @@ struct FormTime {
 };
 constexpr FormTime kProduct16[] = {
     {kLarge, 256, 256, 1, 24.f, 46.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 40.f, 0.6f}, {kSmall, 64, 64, 2, 2.f, 17.f, 0.6f}};
+// (staged through registers: 240 products, 2.5 % over the best on average and at most 1.39 times, 4.7 % and 1.5 by kProduct16)
+constexpr FormTime kStaged16[] = {
+    {kLarge, 256, 256, 1, 0.f, 100.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 70.f, 0.75f}, {kSmall, 64, 64, 2, 0.f, 26.f, 0.75f}};
 constexpr FormTime kGradient16[] = {
     {kLarge, 256, 256, 1, 8.f, 42.f, 1.f}, {kMiddle, 128, 128, 2, 0.f, 42.f, 1.f}, {kSmall, 64, 64, 2, 1.f, 17.f, 1.f}};
 constexpr FormTime kProduct32[] = {
@@ -905,8 +908,8 @@ uint64_t likely_tiles(const bpl_expert_descriptor &d, uint32_t height, uint32_t 
   return (full > met ? full : met) * div_up(d.out, width);
 }
 
-Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
-  return best_form(element_bytes == 2 ? kProduct16 : kProduct32, d.width, worth_quarters(d),
+Form product_form(uint32_t element_bytes, bool staged, const bpl_expert_descriptor &d) {
+  return best_form(element_bytes == 4 ? kProduct32 : staged ? kStaged16 : kProduct16, d.width, worth_quarters(d),
                    [&](uint32_t height, uint32_t width) { return likely_tiles(d, height, width); });
 }
 
@@ -915,7 +918,7 @@ Form product_form(uint32_t element_bytes, const bpl_expert_descriptor &d) {
 // 0.25 us each in 16 bits and 0.35 in 32, and the weights at 5 TB/s.  (One row, 4,096 x 64, bfloat16 19 -> 8 + 4 us; two rows on
 // two experts of 2,048 x 1,024, float32 29 -> 13 + 4, bfloat16 11.3 and left as it is, where it would be 7.7 + 4.)
 uint32_t product_parts(uint32_t element_bytes, const bpl_expert_descriptor &d) {
-  const Form form = product_form(element_bytes, d);
+  const Form form = product_form(element_bytes, false, d);
   if (form != kSmall && form != kThin) return 1;
   const uint32_t height = form == kSmall ? 64 : 16, share = form == kSmall && element_bytes == 2 ? 2 : 3;
   const uint64_t met = d.experts < d.rows ? d.experts : d.rows;
@@ -933,7 +936,7 @@ uint32_t product_parts(uint32_t element_bytes, const bpl_expert_descriptor &d) {
 
 template <typename T, typename SHAPES, typename O>
 bool choose_product(const char *target, hipStream_t stream, Product<O> p) {
-  Form form = product_form(sizeof(T), p.d);
+  Form form = product_form(sizeof(T), std::is_same<SHAPES, Staged>::value, p.d);
   p.split = false;
   if (p.parts != 1 && form != kThin) form = kSmall;
   if constexpr (sizeof(T) == 2 && std::is_same<T, O>::value) {
