@@ -227,9 +227,10 @@ using Sums = typename Unit<T, S::kSide>::acc[S::kFragsM][S::kFragsN];
 
 typedef uint32_t quad32 __attribute__((ext_vector_type(4)));
 // Past the caches.  (As an instruction of its own: of a nontemporal store and a plain one that a branch chooses between, the
-// compiler makes one plain one.  The wait state is for what may overwrite the data's registers next.)
+// compiler makes one plain one.  The two wait states are for a vector instruction that overwrites the data's registers next:
+// a store of more than 64 bits reads them late, and the compiler does not know of one that it does not see.)
 __device__ __forceinline__ void store_past(void *to, quad32 v) {
-  asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 0" ::"v"(to), "v"(v) : "memory");
+  asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" ::"v"(to), "v"(v) : "memory");
 }
 
 // A wave's results to memory by way of a piece of LDS of its own, so that whole pieces of a row go side by side: a lane holds,
