@@ -136,7 +136,7 @@ _MOST_HOST_SCALARS = 4096
 def _bits(t):
   """The bytes of a host tensor of one element."""
   try:
-    return t.numpy().tobytes()
+    return (t.view(torch.int16) if t.dtype == torch.bfloat16 else t).numpy().tobytes()  # (numpy has no bfloat16)
   except RuntimeError:
     if not _is_plain(t):
       raise

@@ -155,3 +155,28 @@ def test_the_plain_gradient_of_the_choice_against_differences(normalize):
       down[t, j] -= h
       slope = ((plain.topk(up, 4, normalize)[0] - plain.topk(down, 4, normalize)[0]) * ct).sum() / (2 * h)
       assert abs(slope - grad[t, j]) < 1e-8
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["plain", "inference", "parameter", "transform"])
+def test_one_element_on_the_host_goes_to_the_device_in_every_type(dtype, kind, monkeypatch):
+  # (the meta device stands for a GPU; the copies are told apart by their values' bits)
+  from brainpylib_amd import _tensors
+  monkeypatch.setattr(_tensors, "_HOST_SCALARS", {})
+  device = torch.device("meta")
+  with torch.inference_mode(kind == "inference"):
+    operands = [torch.full((1, 1), v, dtype=dtype) for v in (1.5, -1.5, 0.0, -0.0, float("nan"))]
+  if kind == "parameter":
+    operands = [torch.nn.Parameter(t, requires_grad=False) for t in operands]
+
+  def move(x):
+    for t in operands:
+      moved = _tensors.to_device(t, device)
+      assert moved.dtype == dtype and moved.shape == (1, 1) and moved.device == device
+      assert _tensors.to_device(t.clone() if kind == "plain" else t, device) is moved
+    return x.sum()
+  if kind == "transform":
+    torch.func.grad(move)(torch.ones(2))
+  else:
+    move(torch.ones(2))
+  assert len(_tensors._HOST_SCALARS) == len(operands)

@@ -667,3 +667,21 @@ def test_captured_sort_of_many_pairs_replays(cuda):
     torch.cuda.synchronize()
     for a, b in zip(got, plain.sort(chosen, 50)):
       assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operands_of_one_element_from_the_host(cuda, dtype):
+  def one(*shape, value=1.5):
+    return torch.full(shape, value, dtype=dtype)
+  weights, chosen = bpl.expert_topk(one(1, 1), k=1)
+  assert weights.tolist() == [[1.0]] and chosen.tolist() == [[0]]
+  indptr, order, position = bpl.expert_sort(chosen.cpu(), num_experts=1)
+  assert (indptr.tolist(), order.tolist(), position.tolist()) == ([0, 1], [0], [[0]])
+  rows = bpl.expert_dispatch(one(1, 1), order.cpu(), position.cpu())
+  out = bpl.expert_matmul(one(1, 1), one(1, 1, 1, value=-2.0), indptr.cpu())
+  back = bpl.expert_combine(one(1, 1, value=-3.0), weights.cpu(), order.cpu(), position.cpu())
+  assert (rows.tolist(), out.tolist(), back.tolist()) == ([[1.5]], [[-3.0]], [[-3.0]])
+  assert rows.dtype == out.dtype == back.dtype == dtype
+  given = one(1, 1).requires_grad_()  # (a gradient goes back to the host)
+  bpl.expert_matmul(given, one(1, 1, 1, value=-2.0), indptr).sum().backward()
+  assert given.grad.device.type == "cpu" and given.grad.tolist() == [[-2.0]]
