@@ -11,7 +11,8 @@ only the products that it names are computed.  The reference has no such operato
     out = expert_combine(rows, weights, order, position)              # the weighted sum of every token's rows
 
 Values are float32, float16 or bfloat16; sums, softmax and routing weights are held in 32 bits.  Gradients are of first
-order, in backward mode.  No call waits for the GPU or reads a count back, so all of them can be captured into a HIP graph;
+order, in backward mode: of ``autograd`` or of ``torch.func.grad`` and ``vjp``.  Forward mode and batches (``jvp``, ``vmap`` and what
+uses it, as ``jacrev`` and ``is_grads_batched`` do) are refused with NotImplementedError.  No call waits for the GPU or reads a count back, so all of them can be captured into a HIP graph;
 none uses scratch memory that outlives it, so graphs share none.  Results do not depend on the order of atomics.
 """
 import torch
@@ -92,29 +93,79 @@ def _differentiable(name, *tensors):
   return wanted and torch.is_grad_enabled()
 
 
-class _FirstOrder(torch.autograd.Function):
-  """A gradient, unchanged, of which no gradient can be had: it takes part in the graph of what it was computed from."""
+# ---- transforms of torch.func -----------------------------------------------------------------------------------------
+# Inside one tensors are wrappers without memory of their own, those that are made there too.  torch looks under them for
+# an autograd function whose context is set up by a step of its own; that step costs 5 us of host time a call, so that
+# functions have it only where a transform is active.
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
+class _Launch(torch.autograd.Function):
+  """launch(*args), of which no gradient can be had: it takes part in the graph of what it is computed from."""
 
   @staticmethod
-  def forward(ctx, name, grad, *sources):
-    ctx.name = name
-    return grad.view_as(grad)
+  def forward(name, launch, *args):
+    return launch(*args)
 
   @staticmethod
-  def backward(ctx, ct):
+  def setup_context(ctx, inputs, output):
+    ctx.name, ctx.inputs = inputs[0], len(inputs)
+    outputs = output if isinstance(output, tuple) else (output,)
+    ctx.mark_non_differentiable(*[t for t in outputs if t is not None and not t.is_floating_point()])
+    ctx.set_materialize_grads(False)
+
+  @staticmethod
+  def backward(ctx, *cts):
+    if all(ct is None for ct in cts):
+      return (None,) * ctx.inputs
     raise NotImplementedError(f'{ctx.name} has gradients of first order only.')
 
+  @staticmethod
+  def vmap(info, in_dims, name, *args):
+    raise NotImplementedError(f'{name} has no rule for batches (vmap).')
 
-def _cotangent(name, ct):
+
+def _launched(name, launch, *args):
+  """launch(*args), on the tensors underneath where a transform is active."""
+  return _Launch.apply(name, launch, *args) if _transforms_active() else launch(*args)
+
+
+def _gradient(name, launch, ct, *args):
+  """launch(ct, *args): gradients, of which none can be had."""
   if has_tangent(ct):
     raise NotImplementedError(f'{name} has no forward-mode differentiation.')
-  return ct.detach().contiguous()
+  if _transforms_active():
+    return _Launch.apply(name, launch, ct, *args)
+  try:
+    ct.data_ptr()
+  except RuntimeError:  # (a batch of cotangents, which is no active transform for the backward pass)
+    raise NotImplementedError(f'{name} has no rule for batches (vmap).') from None
+  return _Launch.apply(name, launch, ct, *args) if torch.is_grad_enabled() else launch(ct, *args)  # (create_graph)
 
 
-def _first_order(name, grad, *sources):
-  if grad is not None and torch.is_grad_enabled() and any(t.requires_grad for t in sources):  # (create_graph)
-    return _FirstOrder.apply(name, grad, *sources)
-  return grad
+class _Operator(torch.autograd.Function):
+  """What the operators' differentiation rules share: the operator's ``name``, its ``launch`` and ``keep``, which sets up the context.
+  Each is made into a second one for transforms, ``inside``."""
+
+  @classmethod
+  def forward(cls, ctx, *inputs):
+    output = cls.launch(*inputs)
+    cls.keep(ctx, inputs, output)
+    return output
+
+  @classmethod
+  def run(cls, *inputs):
+    return (cls.inside if _transforms_active() else cls).apply(*inputs)
+
+
+def _inside_transforms(operator):
+  """Class decorator: adds ``inside``."""
+  def vmap(info, in_dims, *inputs):
+    raise NotImplementedError(f'{operator.name} has no rule for batches (vmap).')
+
+  operator.inside = type(operator.__name__ + 'Inside', (operator,), {
+    'forward': staticmethod(operator.launch), 'setup_context': staticmethod(operator.keep), 'vmap': staticmethod(vmap)})
+  return operator
 
 
 # ---- expert_topk ------------------------------------------------------------------------------------------------------
@@ -128,29 +179,33 @@ def _topk(logits, mask, k, normalize):
   return weights, chosen
 
 
-class _ExpertTopk(torch.autograd.Function):
+def _topk_gradient(ct, logits, chosen, weights, normalize):
+  grad = torch.empty_like(logits)
+  opaque = _lib.build_expert_descriptor(logits.shape[0], chosen.shape[1], logits.shape[1], 0, 0, 0, _NORMALIZE if normalize else 0)
+  _call('expert_topk_gradient' + _TYPE_NAME[logits.dtype], [logits, chosen, weights, ct.contiguous(), grad], opaque)
+  return grad
+
+
+@_inside_transforms
+class _ExpertTopk(_Operator):
   """With w the weights, g their cotangent: normalized, the chosen logits' cotangents are w (g - sum w g) and the others'
   0; else, with p the softmax over all experts, p ([chosen] g - sum w g)."""
+  name = 'expert_topk'
+  launch = staticmethod(_topk)
 
   @staticmethod
-  def forward(ctx, logits, mask, k, normalize):
-    weights, chosen = _topk(logits, mask, k, normalize)
-    ctx.k, ctx.normalize = k, normalize
+  def keep(ctx, inputs, output):
+    logits, _, _, ctx.normalize = inputs
+    weights, chosen = output
     ctx.mark_non_differentiable(chosen)
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(logits, weights, chosen)
-    return weights, chosen
+    ctx.save_for_backward(logits, chosen, weights)
 
   @staticmethod
   def backward(ctx, ct, _):
     if ct is None:
       return None, None, None, None
-    logits, weights, chosen = ctx.saved_tensors
-    given, ct = ct, _cotangent('expert_topk', ct)
-    grad = torch.empty_like(logits)
-    opaque = _lib.build_expert_descriptor(logits.shape[0], ctx.k, logits.shape[1], 0, 0, 0, _NORMALIZE if ctx.normalize else 0)
-    _call('expert_topk_gradient' + _TYPE_NAME[logits.dtype], [logits, chosen, weights, ct, grad], opaque)
-    return _first_order('expert_topk', grad, given, logits), None, None, None
+    return _gradient('expert_topk', _topk_gradient, ct, *ctx.saved_tensors, ctx.normalize), None, None, None
 
 
 def expert_topk(logits, *, k: int, normalize: bool = True, mask=None):
@@ -181,25 +236,13 @@ def expert_topk(logits, *, k: int, normalize: bool = True, mask=None):
       raise ValueError(f'mask should be a bool for each of the {logits.shape[0]} tokens, got {mask.dtype} {tuple(mask.shape)}.')
     logits, mask = _move(logits, mask)
   if _differentiable('expert_topk', logits):
-    return _ExpertTopk.apply(logits, mask, int(k), bool(normalize))
-  return _topk(logits, mask, int(k), bool(normalize))
+    return _ExpertTopk.run(logits, mask, int(k), bool(normalize))
+  return _launched('expert_topk', _topk, logits, mask, int(k), bool(normalize))
 
 
 # ---- expert_sort ------------------------------------------------------------------------------------------------------
-def expert_sort(experts, *, num_experts: int):
-  """Sorts pairs of a token and an expert by expert, in the pairs' order within one.
-
-  experts  (tokens, k) or (pairs,) int32 | uint32; what is outside [0, num_experts) is dropped
-  returns  ``(indptr, order, position)``, int32: expert ``e`` has the rows ``indptr[e]`` to ``indptr[e + 1] - 1``; row ``r``
-           holds pair ``order[r]`` (pairs are numbered row by row), -1 from row ``indptr[num_experts]`` on; pair ``p`` has row
-           ``position.reshape(-1)[p]``, -1 where it was dropped.  ``position`` has the shape of ``experts``."""
-  experts = as_tensor(experts)
-  _check_index('experts', experts, 1 if experts.ndim == 1 else 2)
-  _check_experts(num_experts)
+def _sort(experts, num_experts):
   pairs = experts.numel()
-  if pairs > _MOST:
-    raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
-  experts, = _move(experts)
 
   def ints(*shape):
     return torch.empty(shape, dtype=torch.int32, device=experts.device)
@@ -210,6 +253,22 @@ def expert_sort(experts, *, num_experts: int):
   opaque = _lib.build_expert_descriptor(pairs, 1, num_experts, 0, 0, 0, 0)
   _call('expert_sort', [experts, indptr, order, position, scratch], opaque)
   return indptr, order, position
+
+
+def expert_sort(experts, *, num_experts: int):
+  """Sorts pairs of a token and an expert by expert, in the pairs' order within one.
+
+  experts  (tokens, k) or (pairs,) int32 | uint32; what is outside [0, num_experts) is dropped
+  returns  ``(indptr, order, position)``, int32: expert ``e`` has the rows ``indptr[e]`` to ``indptr[e + 1] - 1``; row ``r``
+           holds pair ``order[r]`` (pairs are numbered row by row), -1 from row ``indptr[num_experts]`` on; pair ``p`` has row
+           ``position.reshape(-1)[p]``, -1 where it was dropped.  ``position`` has the shape of ``experts``."""
+  experts = as_tensor(experts)
+  _check_index('experts', experts, 1 if experts.ndim == 1 else 2)
+  _check_experts(num_experts)
+  if experts.numel() > _MOST:
+    raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
+  experts, = _move(experts)
+  return _launched('expert_sort', _sort, experts, num_experts)
 
 
 # ---- expert_dispatch, expert_combine ----------------------------------------------------------------------------------
@@ -224,25 +283,29 @@ def _dispatch(tokens, order, position):
   return rows
 
 
-class _ExpertDispatch(torch.autograd.Function):
+def _dispatch_gradient(ct, order, position):
+  grad = torch.empty((position.shape[0], ct.shape[1]), dtype=ct.dtype, device=ct.device)
+  _call('expert_dispatch_gradient' + _TYPE_NAME[ct.dtype], [ct.contiguous(), order, position, grad],
+        _pairs_opaque(position, ct.shape[1]))
+  return grad
+
+
+@_inside_transforms
+class _ExpertDispatch(_Operator):
   """The cotangent of a token is the sum of its rows' cotangents."""
+  name = 'expert_dispatch'
+  launch = staticmethod(_dispatch)
 
   @staticmethod
-  def forward(ctx, tokens, order, position):
-    ctx.save_for_backward(order, position)
+  def keep(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[1:])
     ctx.set_materialize_grads(False)
-    return _dispatch(tokens, order, position)
 
   @staticmethod
   def backward(ctx, ct):
     if ct is None:
       return None, None, None
-    order, position = ctx.saved_tensors
-    given, ct = ct, _cotangent('expert_dispatch', ct)
-    grad = torch.empty((position.shape[0], ct.shape[1]), dtype=ct.dtype, device=ct.device)
-    _call('expert_dispatch_gradient' + _TYPE_NAME[ct.dtype], [ct, order, position, grad],
-          _pairs_opaque(position, ct.shape[1]))
-    return _first_order('expert_dispatch', grad, given), None, None
+    return _gradient('expert_dispatch', _dispatch_gradient, ct, *ctx.saved_tensors), None, None
 
 
 def expert_dispatch(tokens, order, position):
@@ -258,8 +321,8 @@ def expert_dispatch(tokens, order, position):
   _check_pairs(order, position, tokens.shape[0])
   tokens, order, position = _move(tokens, order, position)
   if _differentiable('expert_dispatch', tokens):
-    return _ExpertDispatch.apply(tokens, order, position)
-  return _dispatch(tokens, order, position)
+    return _ExpertDispatch.run(tokens, order, position)
+  return _launched('expert_dispatch', _dispatch, tokens, order, position)
 
 
 def _combine(rows, weights, order, position):
@@ -269,29 +332,33 @@ def _combine(rows, weights, order, position):
   return out
 
 
-class _ExpertCombine(torch.autograd.Function):
+def _combine_gradient(ct, rows, weights, order, position, want_rows, want_weights):
+  d_rows = torch.empty_like(rows) if want_rows else None
+  d_weights = torch.empty_like(weights) if want_weights else None
+  opaque = _pairs_opaque(position, rows.shape[1], (_D_ROWS if want_rows else 0) | (_D_WEIGHTS if want_weights else 0))
+  _call('expert_combine_gradient' + _TYPE_NAME[rows.dtype],
+        [rows, weights, order, position, ct.contiguous(), d_rows if want_rows else rows, d_weights if want_weights else weights],
+        opaque)
+  return d_rows, d_weights
+
+
+@_inside_transforms
+class _ExpertCombine(_Operator):
   """The cotangent of a row is its token's times the pair's weight, that of the weight their inner product with the row."""
+  name = 'expert_combine'
+  launch = staticmethod(_combine)
 
   @staticmethod
-  def forward(ctx, rows, weights, order, position):
-    ctx.save_for_backward(rows, weights, order, position)
+  def keep(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
     ctx.set_materialize_grads(False)
-    return _combine(rows, weights, order, position)
 
   @staticmethod
   def backward(ctx, ct):
-    want_rows, want_weights = ctx.needs_input_grad[:2]
-    if ct is None or not (want_rows or want_weights):
+    wanted = ctx.needs_input_grad[:2]
+    if ct is None or not any(wanted):
       return None, None, None, None
-    rows, weights, order, position = ctx.saved_tensors
-    given, ct = ct, _cotangent('expert_combine', ct)
-    d_rows = torch.empty_like(rows) if want_rows else None
-    d_weights = torch.empty_like(weights) if want_weights else None
-    opaque = _pairs_opaque(position, rows.shape[1], (_D_ROWS if want_rows else 0) | (_D_WEIGHTS if want_weights else 0))
-    _call('expert_combine_gradient' + _TYPE_NAME[rows.dtype],
-          [rows, weights, order, position, ct, d_rows if want_rows else rows, d_weights if want_weights else weights], opaque)
-    sources = (given, rows, weights)
-    return _first_order('expert_combine', d_rows, *sources), _first_order('expert_combine', d_weights, *sources), None, None
+    return _gradient('expert_combine', _combine_gradient, ct, *ctx.saved_tensors, *wanted) + (None, None)
 
 
 def expert_combine(rows, weights, order, position):
@@ -315,8 +382,8 @@ def expert_combine(rows, weights, order, position):
     raise ValueError(f'rows should have a row for each entry of order, got {rows.shape[0]} != {order.shape[0]}.')
   rows, weights, order, position = _move(rows, weights, order, position)
   if _differentiable('expert_combine', rows, weights):
-    return _ExpertCombine.apply(rows, weights, order, position)
-  return _combine(rows, weights, order, position)
+    return _ExpertCombine.run(rows, weights, order, position)
+  return _launched('expert_combine', _combine, rows, weights, order, position)
 
 
 # ---- expert_matmul ----------------------------------------------------------------------------------------------------
@@ -332,34 +399,41 @@ def _matmul(rows, stored, indptr, out_major):
   return out
 
 
-class _ExpertMatmul(torch.autograd.Function):
+def _matmul_gradient(ct, rows, indptr, shape, out_major):
+  """The cotangent of the weight as it lies in memory, ``shape``."""
+  d_stored = torch.empty(shape, dtype=rows.dtype, device=rows.device)
+  parts = _lib.expert_matmul_gradient_parts(rows.shape[0], shape[0], rows.shape[1], ct.shape[1], rows.element_size())
+  scratch = d_stored if parts == 1 else torch.empty((parts,) + shape, dtype=torch.float32, device=rows.device)
+  opaque = _lib.build_expert_descriptor(0, parts, shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
+                                        _OUT_MAJOR if out_major else 0)
+  _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct.contiguous(), indptr, d_stored, scratch], opaque)
+  return d_stored
+
+
+@_inside_transforms
+class _ExpertMatmul(_Operator):
   """The rows' cotangent is the product with the transposed weights, the weights' is rows_e^T @ ct_e for every expert."""
+  name = 'expert_matmul'
+  launch = staticmethod(_matmul)
 
   @staticmethod
-  def forward(ctx, rows, stored, indptr, out_major):
-    ctx.out_major = out_major
-    ctx.save_for_backward(rows, stored, indptr)
+  def keep(ctx, inputs, output):
+    ctx.out_major = inputs[3]
+    ctx.save_for_backward(*inputs[:3])
     ctx.set_materialize_grads(False)
-    return _matmul(rows, stored, indptr, out_major)
 
   @staticmethod
   def backward(ctx, ct):
     if ct is None:
       return None, None, None, None
     rows, stored, indptr = ctx.saved_tensors
-    given, ct = ct, _cotangent('expert_matmul', ct)
+    ct = ct.contiguous()
     d_rows = d_stored = None
     if ctx.needs_input_grad[0]:
-      d_rows = _matmul(ct, stored, indptr, not ctx.out_major)
+      d_rows = _gradient('expert_matmul', _matmul, ct, stored, indptr, not ctx.out_major)
     if ctx.needs_input_grad[1]:
-      d_stored = torch.empty_like(stored)
-      parts = _lib.expert_matmul_gradient_parts(rows.shape[0], stored.shape[0], rows.shape[1], ct.shape[1], rows.element_size())
-      scratch = d_stored if parts == 1 else torch.empty((parts,) + tuple(stored.shape), dtype=torch.float32, device=rows.device)
-      opaque = _lib.build_expert_descriptor(0, parts, stored.shape[0], rows.shape[0], rows.shape[1], ct.shape[1],
-                                            _OUT_MAJOR if ctx.out_major else 0)
-      _call('expert_matmul_gradient' + _TYPE_NAME[rows.dtype], [rows, ct, indptr, d_stored, scratch], opaque)
-    sources = (given, rows, stored)
-    return _first_order('expert_matmul', d_rows, *sources), _first_order('expert_matmul', d_stored, *sources), None, None
+      d_stored = _gradient('expert_matmul', _matmul_gradient, ct, rows, indptr, tuple(stored.shape), ctx.out_major)
+    return d_rows, d_stored, None, None
 
 
 def expert_matmul(rows, weight, indptr):
@@ -387,5 +461,5 @@ def expert_matmul(rows, weight, indptr):
   out_major = not weight.is_contiguous() and weight.transpose(1, 2).is_contiguous()
   rows, stored, indptr = _move(rows, weight.transpose(1, 2) if out_major else weight, indptr)
   if _differentiable('expert_matmul', rows, stored):
-    return _ExpertMatmul.apply(rows, stored, indptr, out_major)
-  return _matmul(rows, stored, indptr, out_major)
+    return _ExpertMatmul.run(rows, stored, indptr, out_major)
+  return _launched('expert_matmul', _matmul, rows, stored, indptr, out_major)
