@@ -30,6 +30,11 @@ __device__ __forceinline__ uint2 rows_of(const uint32_t *__restrict__ indptr, ui
   return make_uint2(from, to > from ? to : from);
 }
 
+// The most tiles of `height` rows that any split of the rows into experts has: every expert has at most one that is not full.
+__host__ __device__ constexpr uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
+  return static_cast<uint64_t>(rows) / height + (experts < rows ? experts : rows);
+}
+
 // The experts' rows and where their tiles of `height` rows begin, counted over the experts in their order: in LDS, built
 // by all threads of the workgroup (one barrier, and one for the caller to see it).
 struct Tile {
@@ -39,7 +44,8 @@ struct TileTable {
   uint32_t start[kMostExperts];
   uint32_t wave_total[16];
 
-  // the number of tiles
+  // the number of tiles: of an indptr that is none, no more than the host has counted with (rows that many experts claim would be
+  // worked on again and again, and places beyond 32 bits would never end)
   template <uint32_t THREADS>
   __device__ __forceinline__ uint32_t build(const uint32_t *__restrict__ indptr, uint32_t experts, uint32_t rows, uint32_t height) {
     constexpr uint32_t kPer = (kMostExperts + THREADS - 1) / THREADS, kWaves = THREADS / kWave;
@@ -71,7 +77,8 @@ struct TileTable {
       at += own[j];
     }
     __syncthreads();
-    return uniform(total);
+    const uint64_t most = most_tiles(rows, experts, height);
+    return uniform(total < most ? total : static_cast<uint32_t>(most));
   }
 
   // index < the number of tiles; every wave by itself: the last expert that begins at or before it (those without tiles begin
@@ -91,11 +98,6 @@ struct TileTable {
     return Tile{expert, first, end - first < height ? end : first + height};
   }
 };
-
-uint64_t most_tiles(uint32_t rows, uint32_t experts, uint32_t height) {
-  // every expert has at most one tile that is not full
-  return static_cast<uint64_t>(rows) / height + (experts < rows ? experts : rows);
-}
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
 // One product kernel body for the three products.  C[m][n] = sum over k of A[m][k] B[n][k], tiles of BM x BN, kDepth (128 bytes
