@@ -663,7 +663,10 @@ __global__ __launch_bounds__(256) void combine_gradient_kernel(const T *__restri
 }
 
 // Rows of 64 MB and more are stored past the caches: 131,080 rows of 2,048 bfloat16 114 -> 104 us there, 250 -> 203 us back.
-constexpr uint64_t kPastCaches = 64ull << 20;
+// Where lines of 128 bytes are shared by rows, which then meet in the last cache, only what that does not hold (of the gradients,
+// d_rows and d_weights, past the caches and not: rows of 1,000 bfloat16, 180 MB 102 and 96 us, 400 MB 220 and 235; of 2,052 float32,
+// 240 MB 120 and 103, 400 MB 201 and 212 us; d_rows alone there 73 and 54, of 516 float32, 800 MB, 267 and 386).
+constexpr uint64_t kPastCaches = 64ull << 20, kPastCachesShared = 256ull << 20;
 
 template <typename T>
 uint32_t chunks_of(uint32_t width) { return div_up(width, kWave * Piece<T>::kElems); }
@@ -725,7 +728,8 @@ void combine_gradient(const char *target, hipStream_t stream, void **buffers, co
   if (pairs == 0 || (d_rows == nullptr && d_weights == nullptr)) return;
   const uint32_t zero_groups = d_rows != nullptr ? capped(div_up(pairs, kZeroRows * 4)) : 0u;
   const bool whole = d.width % Piece<T>::kElems == 0;
-  const bool past = static_cast<uint64_t>(pairs) * d.width * sizeof(T) >= kPastCaches;
+  const bool lines = d.width * sizeof(T) % 128 == 0 && reinterpret_cast<uintptr_t>(buffers[5]) % 128 == 0;
+  const bool past = static_cast<uint64_t>(pairs) * d.width * sizeof(T) >= (lines ? kPastCaches : kPastCachesShared);
   const auto kernel = !whole ? &combine_gradient_kernel<T, false, false>
                       : past ? &combine_gradient_kernel<T, true, true> : &combine_gradient_kernel<T, true, false>;
   hipLaunchKernelGGL(kernel, dim3(capped(d.tokens) + zero_groups), dim3(256), 0, stream,

@@ -37,3 +37,26 @@ def test_largest_tiles_stored_past_the_caches(cuda, dtype, out_major):
       assert torch.equal(d_rows[at], (c @ w.t().contiguous()).to(dtype)), (seed, e)
       assert torch.equal(d_weight[e], (x.t().contiguous() @ c).to(dtype)), (seed, e)
     assert (got[indptr[-1]:] == 0).all() and (d_rows[indptr[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype, width, megabytes", [(torch.bfloat16, 1000, 70), (torch.bfloat16, 1000, 300), (torch.float32, 516, 140),
+                                                     (torch.float32, 516, 270), (torch.float16, 1024, 70)])
+def test_gradients_of_combine_of_rows_that_share_lines(cuda, dtype, width, megabytes):
+  # rows that end within a line of 128 bytes, below and above what the last cache holds, and rows that do not
+  k = 4
+  tokens = (megabytes << 20) // (k * width * dtype.itemsize) + 1
+  pairs = tokens * k
+  g = torch.Generator(device="cuda").manual_seed(width)
+  order = torch.randperm(pairs, generator=g, device="cuda").to(torch.int32)
+  position = torch.empty_like(order)
+  position[order.long()] = torch.arange(pairs, dtype=torch.int32, device="cuda")
+  # whole numbers: every product and sum is exact
+  rows = torch.randint(-2, 3, (pairs, width), generator=g, device="cuda").to(dtype).requires_grad_()
+  weights = torch.randint(-3, 4, (tokens, k), generator=g, device="cuda").float().requires_grad_()
+  ct = torch.randint(-2, 3, (tokens, width), generator=g, device="cuda").to(dtype)
+  out = bpl.expert_combine(rows, weights, order, position.reshape(tokens, k))
+  d_rows, d_weights = torch.autograd.grad(out, (rows, weights), ct)
+  at = order.long()
+  assert torch.equal(d_rows, (ct[at // k].float() * weights.detach().reshape(-1)[at][:, None]).to(dtype))
+  picked = rows.detach()[position.long()].reshape(tokens, k, width).float()
+  assert torch.equal(d_weights, (picked * ct[:, None].float()).sum(2))
