@@ -101,7 +101,8 @@ _transforms_active = torch._C._are_functorch_transforms_active
 
 
 class _Launch(torch.autograd.Function):
-  """launch(*args), of which no gradient can be had: it takes part in the graph of what it is computed from."""
+  """launch(*args), on the tensors underneath where a transform is active.  No gradient can be had of it: it takes part in the
+  graph of what it is computed from."""
 
   @staticmethod
   def forward(name, launch, *args):
@@ -123,11 +124,6 @@ class _Launch(torch.autograd.Function):
   @staticmethod
   def vmap(info, in_dims, name, *args):
     raise NotImplementedError(f'{name} has no rule for batches (vmap).')
-
-
-def _launched(name, launch, *args):
-  """launch(*args), on the tensors underneath where a transform is active."""
-  return _Launch.apply(name, launch, *args) if _transforms_active() else launch(*args)
 
 
 def _gradient(name, launch, ct, *args):
@@ -237,19 +233,19 @@ def expert_topk(logits, *, k: int, normalize: bool = True, mask=None):
     logits, mask = _move(logits, mask)
   if _differentiable('expert_topk', logits):
     return _ExpertTopk.run(logits, mask, int(k), bool(normalize))
-  return _launched('expert_topk', _topk, logits, mask, int(k), bool(normalize))
+  if _transforms_active():
+    return _Launch.apply('expert_topk', _topk, logits, mask, int(k), bool(normalize))
+  return _topk(logits, mask, int(k), bool(normalize))
 
 
 # ---- expert_sort ------------------------------------------------------------------------------------------------------
 def _sort(experts, num_experts):
-  pairs = experts.numel()
-
-  def ints(*shape):
-    return torch.empty(shape, dtype=torch.int32, device=experts.device)
-
-  indptr, order, position = ints(num_experts + 1), ints(pairs), ints(*experts.shape)
+  pairs, device = experts.numel(), experts.device
+  indptr = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
+  order = torch.empty(pairs, dtype=torch.int32, device=device)
+  position = torch.empty(experts.shape, dtype=torch.int32, device=device)
   room = _lib.expert_sort_scratch_bytes(pairs, num_experts)
-  scratch = ints(room // 4) if room else indptr  # (not used)
+  scratch = torch.empty(room // 4, dtype=torch.int32, device=device) if room else indptr  # (not used)
   opaque = _lib.build_expert_descriptor(pairs, 1, num_experts, 0, 0, 0, 0)
   _call('expert_sort', [experts, indptr, order, position, scratch], opaque)
   return indptr, order, position
@@ -268,7 +264,9 @@ def expert_sort(experts, *, num_experts: int):
   if experts.numel() > _MOST:
     raise ValueError('Only support up to 2^31 - 1 pairs of a token and an expert.')
   experts, = _move(experts)
-  return _launched('expert_sort', _sort, experts, num_experts)
+  if _transforms_active():
+    return _Launch.apply('expert_sort', _sort, experts, num_experts)
+  return _sort(experts, num_experts)
 
 
 # ---- expert_dispatch, expert_combine ----------------------------------------------------------------------------------
@@ -322,7 +320,9 @@ def expert_dispatch(tokens, order, position):
   tokens, order, position = _move(tokens, order, position)
   if _differentiable('expert_dispatch', tokens):
     return _ExpertDispatch.run(tokens, order, position)
-  return _launched('expert_dispatch', _dispatch, tokens, order, position)
+  if _transforms_active():
+    return _Launch.apply('expert_dispatch', _dispatch, tokens, order, position)
+  return _dispatch(tokens, order, position)
 
 
 def _combine(rows, weights, order, position):
@@ -383,7 +383,9 @@ def expert_combine(rows, weights, order, position):
   rows, weights, order, position = _move(rows, weights, order, position)
   if _differentiable('expert_combine', rows, weights):
     return _ExpertCombine.run(rows, weights, order, position)
-  return _launched('expert_combine', _combine, rows, weights, order, position)
+  if _transforms_active():
+    return _Launch.apply('expert_combine', _combine, rows, weights, order, position)
+  return _combine(rows, weights, order, position)
 
 
 # ---- expert_matmul ----------------------------------------------------------------------------------------------------
@@ -462,4 +464,6 @@ def expert_matmul(rows, weight, indptr):
   rows, stored, indptr = _move(rows, weight.transpose(1, 2) if out_major else weight, indptr)
   if _differentiable('expert_matmul', rows, stored):
     return _ExpertMatmul.run(rows, stored, indptr, out_major)
-  return _launched('expert_matmul', _matmul, rows, stored, indptr, out_major)
+  if _transforms_active():
+    return _Launch.apply('expert_matmul', _matmul, rows, stored, indptr, out_major)
+  return _matmul(rows, stored, indptr, out_major)
