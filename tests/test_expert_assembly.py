@@ -125,3 +125,49 @@ def test_scalar_addresses_are_written_in_time(assembly):
   code = instructions(assembly["expert_matmul.hip"])
   assert sum(i[3] and i[1].startswith("global_load_lds") for i in code) > 100
   assert not early_scalar_reads(code)
+
+
+def test_what_the_loads_to_lds_are_told_is_nothing_elses(assembly):
+  # (m0 is reserved: the compiler takes no note of an assembly statement that writes it, and must have no use of its own for it)
+  for source, text in assembly.items():
+    assert not [i for i in instructions(text) if not i[3] and any("m0" in o.split() for o in i[2])], source
+
+
+# Vector registers that the kernels of the largest tiles spill, at most: (part of the mangled name, registers).  The main loop has
+# none of it, the way of the results out has.
+SPILLS = [(r"14product_kernelI.*Lb1ENS_5ShapeILj256ELj256ELj2ELj2E.*ES2_EEv", 72),
+          (r"14product_kernelI.*Lb0ENS_5ShapeILj256ELj256ELj2ELj2E.*ES2_EEv", 116),
+          (r"14product_kernelI.*Lb[01]ENS_5ShapeILj256ELj256ELj2ELj4E.*ES2_EEv", 24),
+          (r"15gradient_kernelI.*NS_5ShapeILj256ELj256ELj2ELj2E", 60)]
+
+
+def kernels(text):
+  """[(mangled name, bytes of scratch memory a lane, vector registers spilled)]"""
+  pattern = r"\.name:\s+(\S+)\n(?:.*\n)*?\s+\.private_segment_fixed_size:\s+(\d+)\n(?:.*\n)*?\s+\.vgpr_spill_count:\s+(\d+)"
+  return [(n, int(b), int(r)) for n, b, r in re.findall(pattern, text[text.index("amdhsa.kernels"):])]
+
+
+def test_only_the_largest_tiles_spill(assembly):
+  seen, over = 0, []
+  for text in assembly.values():
+    for name, scratch, spilled in kernels(text):
+      most = max([n for part, n in SPILLS if re.search(part, name)], default=0)
+      seen += 1
+      if spilled > most or (most == 0 and scratch):
+        over.append("%s: %d registers, %d bytes a lane" % (name, spilled, scratch))
+  assert seen > 100 and not over, over
+
+
+def test_the_main_loop_of_the_largest_tiles_does_not_spill(assembly):
+  # somewhere a stage's 64 matrix instructions (four steps of 4 x 4; 32 of the waves that take 128 x 64) follow each other with no
+  # spilled register stored or fetched between them
+  text, seen = assembly["expert_matmul.hip"], 0
+  for name, scratch, _ in kernels(text):
+    if not scratch:
+      continue
+    begin = text.index("\n%s:" % name)
+    code = instructions(text[begin:text.index("s_endpgm", begin)])
+    runs = "".join("m" if i[1].startswith("v_mfma") else "s" if i[1].startswith("scratch_") else "" for i in code).split("s")
+    assert max(map(len, runs)) >= (32 if "ILj256ELj256ELj2ELj4E" in name else 64), name
+    seen += 1
+  assert seen >= 6
