@@ -347,7 +347,9 @@ __device__ __forceinline__ void tile_product(const T *__restrict__ a, uint32_t r
 // (Instructions of 16 x 16 take the stage in two steps, each twice as deep.)
 // Loads and reads go between the matrix instructions, evenly: loads in one go hold up the wave that issues them, and a SIMD
 // may have no other.  (Stages of 64 bytes with four places leave the loads the same time, but ask the L2 twice as often.)
-// A tile's results go out by way of room of their own while the next tile's stages come in.
+// A tile's results go out by way of room of their own while the next tile's stages come in.  The 256 x 256 tiles do so in part only:
+// the compiler works out the addresses there ahead of the loop over the tiles and has no registers for them (57 to 112 a lane are
+// spilled, none in the loop over the stages), and what is fetched back waits for every load and store before it.
 //
 // Why these tiles: a wave of 128 x 128 results reads 64 bytes of LDS a cycle and CU for what the matrix unit does, of the 128
 // that LDS gives (64 x 64: 128, which is why smaller tiles are slower: 1,140 / 850 / 480 TFLOP/s for 256 / 128 / 64 squared,
@@ -854,7 +856,8 @@ bool launch_product(const char *target, hipStream_t stream, const Product<O> &p)
 
 // Which shape: the least time by the turns in which the card, full of them, works through a shape's tiles.  A turn's time, in us:
 // `fixed` and, for 2,048 of the inner dimension (in the gradient: of rows to an expert), `deep`; the large shape has one
-// workgroup to a CU, so that nothing goes on there while a tile begins and ends.  `alone`: of a turn that leaves every CU at most
+// workgroup to a CU, so that nothing goes on there while a tile begins and ends, and spilled registers hold up its results (the
+// results' 33 MB of a turn take 7 of the 24 us).  `alone`: of a turn that leaves every CU at most
 // one workgroup where two could share it; of a fuller one the share that its tiles have.
 // Fitted to 528 products in 16 bits (32 and 128 experts, inner dimensions of 1,024 to 8,192, 768 to 2,048 columns, both
 // storages, 4 to 800 rows to an expert) and 144 gradients (8 to 128 experts, 16 to 4,096 rows to one), every shape timed at each:

@@ -44,7 +44,7 @@ __device__ __forceinline__ float group_add(float v) {
 // ---- expert_topk ----------------------------------------------------------------------------------------------------
 // k turns of: the largest key of a lane's 8 logits, of the row's lanes, the lowest place that holds it, that place's key to 0.
 // A row to as few lanes as hold it, so that a wave takes 1 to 8 rows at once and most exchanges are DPP moves.  Bound by
-// instructions, 50 a turn and wave: 32,771 rows of 128 float logits, k = 8, 12 us (1.4 TB/s), its gradient 10.5 us.
+// instructions, 50 a turn and wave: 32,771 rows of 128 float logits, k = 8, 11.4 us (1.5 TB/s), its gradient 10.6 us.
 // Keys whose order as whole numbers is that of the logits: NaN above every number, -0 equal to 0, and 0 for -inf (and
 // for what is beyond the row or taken already), which is never chosen.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -262,7 +262,7 @@ void topk_gradient(const char *target, hipStream_t stream, void **buffers, const
 // its own, scans the experts and ranks its pairs 64 at a time, in their order.  What is dropped counts as one more
 // expert behind the last.  No atomics but in counts, so the result never depends on an order.
 // Bound by the chain of its steps, not by bytes: 524,296 pairs over 256 experts 14.1 us, in two
-// launches of 4.8 and 11 (14.8 with eight rows of counts and no next steps under way).
+// launches of 3.1 and 11.8 (14.8 with eight rows of counts and no next steps under way).
 constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / kWave;
 constexpr uint32_t kSortPairs = 2048;  // to a workgroup, at least
 constexpr uint32_t kSortOne = 8192;    // so many pairs one workgroup takes alone
